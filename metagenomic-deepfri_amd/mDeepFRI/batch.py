@@ -18,10 +18,19 @@ import numpy as np
 
 from . import _hip
 
+# torch comes in with this module, before anything here can make the library's first HIP call: once the HIP runtime is up, `import torch`
+# reads and registers every fat binary of its libraries eagerly instead of on demand (2.5 s with a warm page cache, minutes on a machine
+# that has not read them yet -- tests/conftest.py, pytest_collection_finish), which a process that builds a Predictor first would pay.
+try:
+    import torch as _torch_module
+except ImportError:          # host-side packing and planning need no torch
+    _torch_module = None
+
 
 def _torch():
-    import torch
-    return torch
+    if _torch_module is None:
+        raise ImportError("mDeepFRI.batch needs PyTorch-ROCm for device memory and streams")
+    return _torch_module
 
 
 # ---------------------------------------------------------------------------------------------------------------------
