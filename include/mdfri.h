@@ -232,6 +232,97 @@ int mdf_cnn_forward_dev(mdf_cnn *m, const uint8_t *seq_idx, const int32_t *Lq, c
                         float *scores, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Operators of a state-space language-model block, over packed residue rows (inference).  The reference has no code for them: they stand
+ * beside the recurrent and convolutional sequence models above for features that come from a block of
+ *     pre-norm -> in-projection -> short causal convolution -> selective scan -> gated norm -> out-projection -> post-norm, gate, residual
+ * whose two projections are the caller's own products.
+ *
+ * Sequence b owns rows [row_off[b], row_off[b] + lengths[b]) of R; row_off is ascending (mdf_layout_rows builds one; dense packing is as good)
+ * and a length may be 0.  Rows of no sequence are neither read nor written.  `max_len` is the longest sequence (it sizes the split of long
+ * sequences over workgroups, not the result: a longer one is still run to its end).
+ * Kept states: `slots[b]` (NULL: b) says which of the n_slots states sequence b continues and leaves behind, `positions[b]` (NULL: 0) how many tokens
+ * it had before this call; at position 0 the old state is not read.  A sequence whose slot lies outside [0, n_slots) is skipped: its rows and
+ * every state stay as they are (a padded batch).  The slots of one call must differ; the caller counts the positions.
+ * Types: MDF_DT_F32, MDF_DT_BF16 or MDF_DT_F16 for activations; weights, decays and states are f32, except the convolution's state (raw inputs). */
+#define MDF_DT_BF16 5
+#define MDF_DT_F16 6
+typedef struct {
+    const int32_t *lengths;      /* (B) device */
+    const int32_t *row_off;      /* (B+1) device */
+    const int32_t *slots;        /* (B) device, or NULL */
+    const int32_t *positions;    /* (B) device, or NULL */
+    int64_t R;
+    int32_t B, max_len, n_slots;
+} mdf_seq_rows;
+
+/* out[t][c] = act(bias[c] + sum_k weight[k][c] * x[t - (width-1) + k][c]) along every sequence, act = silu or none; inputs before the sequence's
+ * first token are 0.  state (n_slots, width, channels), of x's type: the input of token t (counted over all calls) is kept at entry
+ * t mod width.  out must not overlap x.  width 1..8. */
+typedef struct {
+    mdf_seq_rows rows;
+    const void *x;
+    const float *weight, *bias;  /* (width, channels); (channels) or NULL */
+    void *state;                 /* or NULL */
+    void *out;
+    int64_t ldx, ldo;            /* row strides in elements */
+    int32_t channels, width, dtype, silu;
+} mdf_conv_args;
+int mdf_causal_conv_dev(const mdf_conv_args *args, void *stream);
+
+/* With D = softplus(dt[t][h] + dt_bias[h]) and g = h / (heads / groups):
+ *     H[p][n] <- exp(D a[h]) H[p][n] + D x[t][h][p] b[t][g][n],     y[t][h][p] = sum_n H[p][n] c[t][g][n] + d[h] x[t][h][p]
+ * over every sequence; H is f32, state (n_slots, heads, head_dim, state_dim).  x, y: (R, heads, head_dim), b, c: (R, groups, state_dim), each
+ * contiguous inside a row; dt (R, heads) of any of the three types.  y must not overlap an input.  head_dim 1..256, state_dim 1..128.
+ * Non-finite values stay where the recurrence puts them: nothing before the token or beside the channel they enter by is touched (an
+ * infinity may come out as NaN). */
+typedef struct {
+    mdf_seq_rows rows;
+    const void *x, *b, *c, *dt;
+    const float *a, *d, *dt_bias;   /* (heads) each; d, dt_bias may be NULL (0) */
+    float *state;                   /* or NULL */
+    void *y;
+    int64_t ldx, ldb, ldc, lddt, ldy;
+    int32_t heads, groups, head_dim, state_dim, dtype, dt_dtype;
+} mdf_scan_args;
+size_t mdf_scan_workspace_bytes(const mdf_scan_args *args);
+int mdf_selective_scan_dev(const mdf_scan_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One token of each of B sequences through the convolution (silu) and the scan, in one launch: xbc (B, heads*head_dim + 2*groups*state_dim) holds
+ * [x | b | c] before the convolution; both states are updated in place; y (B, heads, head_dim).  The convolved values are not rounded to the
+ * activations' type in between.  rows of mdf_seq_rows are the B tokens themselves: lengths / row_off are not used. */
+typedef struct {
+    const void *xbc, *dt;
+    const float *conv_weight, *conv_bias, *a, *d, *dt_bias;
+    void *conv_state;
+    float *state;
+    const int32_t *slots, *positions;
+    void *y;
+    int64_t ldx, lddt, ldy;
+    int32_t B, n_slots, heads, groups, head_dim, state_dim, width, dtype, dt_dtype;
+} mdf_step_args;
+int mdf_selective_step_dev(const mdf_step_args *args, void *stream);
+
+/* Norms before and after a block with its gate, residual scale and residual, one pass over the rows:
+ *     v = s [* act(gate)]      when gate_first          v = post(v)   when post_weight      v = v * act(gate)   when a gate and not gate_first
+ *     r = residual + scale * scale_vec * v   when residual (-> residual_out)                out = pre(r)   when pre_weight,  else v without a residual
+ * post and pre divide by sqrt(mean square + eps) (center: after the mean is taken off), times weight, plus bias; post works on `groups` equal
+ * parts of a row on their own.  groups > 1 needs pre_weight == NULL.  Everything between the inputs and the one rounding of each output is f32.
+ * residual_dtype: f32 or the dtype of s.  An output may BE an input (same address, stride and type), not overlap one otherwise. */
+#define MDF_ACT_NONE 0
+#define MDF_ACT_SILU 1
+#define MDF_ACT_SIGMOID 2
+typedef struct {
+    const void *s, *gate, *residual;
+    const float *post_weight, *post_bias, *pre_weight, *pre_bias, *scale_vec;   /* (dim) each, or NULL */
+    void *residual_out, *out;
+    int64_t lds, ldg, ldr, ldro, ldo;
+    int64_t rows;
+    int32_t dim, groups, dtype, residual_dtype, gate_act, gate_first, center;
+    float scale, eps;
+} mdf_block_norm_args;
+int mdf_block_norm_dev(const mdf_block_norm_args *args, void *stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Batched device API (the counterpart of pipeline.py:476-481 Pool.map(build_align_contact_map) and
  * pipeline.py:292-319 _run_prediction_loop, for B proteins at once).
  *

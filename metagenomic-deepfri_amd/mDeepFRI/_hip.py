@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("MDFRI_HIP_LIB", os.path.join(os.path.dirname(_PKG_DIR
 
 MDF_OK, MDF_EINVAL, MDF_ENODEVICE, MDF_ENOMEM, MDF_EBADCHAR, MDF_ECAPACITY, MDF_EIO = 0, -1, -2, -3, -4, -5, -6
 MDF_PLAN_KEEP_ORDER = 1      # mdf_plan_create_ex flag: visit the proteins as given, not shortest first
-DT_I32, DT_F32, DT_I64, DT_F64, DT_U8 = 0, 1, 2, 3, 4
+DT_I32, DT_F32, DT_I64, DT_F64, DT_U8, DT_BF16, DT_F16 = 0, 1, 2, 3, 4, 5, 6
 
 
 class MdfriError(RuntimeError):
@@ -209,6 +209,12 @@ SIGNATURES = {
     "mdf_matrix_format_host": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_int, _i64p]),
     "mdf_results_format_host": (c_int, [c_void_p, c_void_p, c_char_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                         c_int32, c_int32, c_void_p, c_int64, _i64p, _i64p]),
+    # the state-space block's operators (argument structures by pointer: mDeepFRI/ssm.py)
+    "mdf_causal_conv_dev": (c_int, [c_void_p, c_void_p]),
+    "mdf_scan_workspace_bytes": (c_size_t, [c_void_p]),
+    "mdf_selective_scan_dev": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mdf_selective_step_dev": (c_int, [c_void_p, c_void_p]),
+    "mdf_block_norm_dev": (c_int, [c_void_p, c_void_p]),
     "mdf_timing_enable": (c_int, [c_int]),
     "mdf_timing_read": (c_int, [c_char_p, _i64p, POINTER(c_double)]),
     "mdf_timing_reset": (c_int, []),

@@ -1,0 +1,323 @@
+"""Operators of a state-space language-model block over packed residue rows (include/mdfri.h "Operators of a state-space language-model block"):
+
+    causal_conv      the short causal convolution along every sequence
+    selective_scan   the recurrence  H <- exp(D a) H + D x (x) b,  y = H c + d x  along every sequence
+    selective_step   both for ONE token of each of many sequences, in one launch
+    block_norm       the norms before and after a block with its gate, residual scale and residual
+
+They stand beside the recurrent and convolutional sequence models of this package (mDeepFRI.predict: LSTM branch, CNN) for features of a block
+    x -> pre-norm -> in-projection -> causal_conv -> selective_scan -> block_norm(gate=z, gate_first=True) -> out-projection -> block_norm(residual=...)
+whose two projections are products of the caller's.  The reference has nothing of the kind; inference only: a tensor that asks for a gradient
+is refused.
+
+Tensors are torch tensors on one GPU; work is enqueued on that GPU's current stream and nothing waits for it.  Rows of no sequence are
+left as they were in an `out` that is handed in and are zero in one that is made here.  Outputs are f32, bfloat16 or float16 like their
+inputs, everything in between is f32."""
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_float, c_int32, c_int64, c_void_p
+
+import numpy as np
+
+from . import _hip
+from .batch import _torch
+
+ACTS = {"none": 0, "silu": 1, "sigmoid": 2}
+
+
+class _Rows(ctypes.Structure):
+    _fields_ = [("lengths", c_void_p), ("row_off", c_void_p), ("slots", c_void_p), ("positions", c_void_p), ("R", c_int64), ("B", c_int32), ("max_len", c_int32),
+                ("n_slots", c_int32)]
+
+
+class _Conv(ctypes.Structure):
+    _fields_ = [("rows", _Rows), ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("state", c_void_p), ("out", c_void_p), ("ldx", c_int64), ("ldo", c_int64),
+                ("channels", c_int32), ("width", c_int32), ("dtype", c_int32), ("silu", c_int32)]
+
+
+class _Scan(ctypes.Structure):
+    _fields_ = [("rows", _Rows), ("x", c_void_p), ("b", c_void_p), ("c", c_void_p), ("dt", c_void_p), ("a", c_void_p), ("d", c_void_p), ("dt_bias", c_void_p), ("state", c_void_p),
+                ("y", c_void_p), ("ldx", c_int64), ("ldb", c_int64), ("ldc", c_int64), ("lddt", c_int64), ("ldy", c_int64), ("heads", c_int32), ("groups", c_int32),
+                ("head_dim", c_int32), ("state_dim", c_int32), ("dtype", c_int32), ("dt_dtype", c_int32)]
+
+
+class _Step(ctypes.Structure):
+    _fields_ = [("xbc", c_void_p), ("dt", c_void_p), ("conv_weight", c_void_p), ("conv_bias", c_void_p), ("a", c_void_p), ("d", c_void_p), ("dt_bias", c_void_p),
+                ("conv_state", c_void_p), ("state", c_void_p), ("slots", c_void_p), ("positions", c_void_p), ("y", c_void_p), ("ldx", c_int64), ("lddt", c_int64), ("ldy", c_int64),
+                ("B", c_int32), ("n_slots", c_int32), ("heads", c_int32), ("groups", c_int32), ("head_dim", c_int32), ("state_dim", c_int32), ("width", c_int32), ("dtype", c_int32),
+                ("dt_dtype", c_int32)]
+
+
+class _Norm(ctypes.Structure):
+    _fields_ = [("s", c_void_p), ("gate", c_void_p), ("residual", c_void_p), ("post_weight", c_void_p), ("post_bias", c_void_p), ("pre_weight", c_void_p), ("pre_bias", c_void_p),
+                ("scale_vec", c_void_p), ("residual_out", c_void_p), ("out", c_void_p), ("lds", c_int64), ("ldg", c_int64), ("ldr", c_int64), ("ldro", c_int64), ("ldo", c_int64),
+                ("rows", c_int64), ("dim", c_int32), ("groups", c_int32), ("dtype", c_int32), ("residual_dtype", c_int32), ("gate_act", c_int32), ("gate_first", c_int32),
+                ("center", c_int32), ("scale", c_float), ("eps", c_float)]
+
+
+_DTYPES = None
+
+
+def _dtype(t, name: str) -> int:
+    global _DTYPES
+    if _DTYPES is None:
+        torch = _torch()
+        _DTYPES = {torch.float32: _hip.DT_F32, torch.bfloat16: _hip.DT_BF16, torch.float16: _hip.DT_F16}
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: {t.dtype} is not float32, bfloat16 or float16")
+    return code
+
+
+class SequenceRows:
+    """Which rows belong to which sequence: `lengths` (B) and `row_off` (B+1), int32 device tensors, row_off ascending, and the longest length.
+    `dense`: the sequences cover every row (an output made here then needs no zeros).  `build` makes one from host lengths and checks them."""
+
+    __slots__ = ("lengths", "row_off", "max_len", "dense")
+
+    def __init__(self, lengths, row_off, max_len: int, dense: bool = False):
+        torch = _torch()
+        if lengths.dtype != torch.int32 or row_off.dtype != torch.int32 or lengths.dim() != 1 or row_off.dim() != 1 or not lengths.is_contiguous() or not row_off.is_contiguous():
+            raise ValueError("lengths and row_off must be contiguous one-dimensional int32 tensors")
+        if row_off.shape[0] != lengths.shape[0] + 1:
+            raise ValueError(f"row_off has {row_off.shape[0]} entries for {lengths.shape[0]} sequences (one more is wanted)")
+        if lengths.device != row_off.device or max_len < 0:
+            raise ValueError("lengths and row_off lie on different devices, or max_len is negative")
+        self.lengths, self.row_off, self.max_len, self.dense = lengths, row_off, int(max_len), dense
+
+    @classmethod
+    def build(cls, lengths, device="cuda", align: int = 1):
+        """From host lengths; `align` rounds every sequence's first row up (_hip: MDF_GROUP_ROWS = 16 gives the rows of mdf_layout_rows)."""
+        torch = _torch()
+        n = np.asarray(lengths, dtype=np.int64)
+        if n.ndim != 1 or (n < 0).any() or align < 1:
+            raise ValueError("lengths must be a list of counts, none negative")
+        off = np.zeros(len(n) + 1, dtype=np.int64)
+        np.cumsum(-(-n // align) * align, out=off[1:])
+        if off[-1] >= 2**31:
+            raise ValueError("too many rows for int32 offsets; split the batch")
+        return cls(torch.from_numpy(n.astype(np.int32)).to(device), torch.from_numpy(off.astype(np.int32)).to(device), int(n.max(initial=0)), dense=bool(off[-1] == n.sum()))
+
+
+def check_slots(slots, n_slots: int, device="cuda"):
+    """Host list of state slots -> int32 device tensor; refuses one that is named twice or lies outside the pool (negative ones, which skip
+    their sequence, may repeat)."""
+    torch = _torch()
+    s = np.asarray(slots, dtype=np.int64)
+    live = s[s >= 0]
+    if s.ndim != 1 or (live >= n_slots).any():
+        raise ValueError(f"a slot lies outside the {n_slots} states")
+    if len(np.unique(live)) != len(live):
+        raise ValueError("two sequences share a state slot")
+    return torch.from_numpy(s.astype(np.int32)).to(device)
+
+
+def _matrix(t, name: str, device, tail: tuple, rows=None):
+    """Checks a tensor of `rows` rows whose trailing dimensions are `tail`, contiguous inside a row; returns its row stride."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} is not on a GPU")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.requires_grad and _torch().is_grad_enabled():
+        raise ValueError(f"{name} asks for a gradient: the state-space operators are inference only")
+    if tuple(t.shape[1:]) != tail or (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, wanted {(rows if rows is not None else '*',) + tail}")
+    want = 1
+    for size, stride in zip(reversed(tail), reversed(t.stride()[1:])):
+        if size != 1 and stride != want:
+            raise ValueError(f"{name}: strides {t.stride()}: only the row stride is free")
+        want *= size
+    return t.stride(0)
+
+
+def _vector(t, name: str, device, shape: tuple):
+    """Checks an f32 parameter; returns its address (None: NULL)."""
+    if t is None:
+        return None
+    if t.dtype != _torch().float32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor of shape {shape} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.requires_grad and _torch().is_grad_enabled():
+        raise ValueError(f"{name} asks for a gradient: the state-space operators are inference only")
+    return t.data_ptr()
+
+
+def _indices(t, name: str, device, count: int):
+    if t is None:
+        return None
+    if t.dtype != _torch().int32 or t.shape != (count,) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {count} entries on {device}")
+    return t.data_ptr()
+
+
+def _state(t, name: str, device, dtype, tail: tuple):
+    if t.dtype != dtype or tuple(t.shape[1:]) != tail or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {('*',) + tail} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _fill_rows(r: _Rows, rows: SequenceRows, device, total: int, slots, positions, state) -> None:
+    if state is None and (slots is not None or positions is not None):
+        raise ValueError("slots and positions belong to a kept state: none is given")
+    if rows.lengths.device != device:
+        raise ValueError(f"lengths are on {rows.lengths.device}, not on {device}")
+    n = rows.lengths.shape[0]
+    r.lengths, r.row_off, r.R, r.B, r.max_len = rows.lengths.data_ptr(), rows.row_off.data_ptr(), total, n, rows.max_len
+    r.slots, r.positions = _indices(slots, "slots", device, n), _indices(positions, "positions", device, n)
+    r.n_slots = 0 if state is None else state.shape[0]
+
+
+def _made(out, like, rows: SequenceRows, shape):
+    if out is None:
+        torch = _torch()
+        return torch.empty(shape, dtype=like.dtype, device=like.device) if rows.dense else torch.zeros(shape, dtype=like.dtype, device=like.device)
+    if out.dtype != like.dtype:
+        raise ValueError(f"out is {out.dtype}, the input {like.dtype}")
+    return out
+
+
+def _call(fn, device, *args) -> None:
+    """Runs a library entry on the device's current stream, with that device current."""
+    torch = _torch()
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        _hip.check(fn(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            _hip.check(fn(*args, stream))
+
+
+def causal_conv(x, weight, rows: SequenceRows, *, bias=None, silu: bool = True, state=None, slots=None, positions=None, out=None):
+    """out[t, c] = act(bias[c] + sum_k weight[k, c] x[t - (width-1) + k, c]) along every sequence; inputs before a sequence's first token are 0.
+
+    x (R, channels), any row stride; weight (width, channels) and bias (channels) f32, width 1..8; silu: the activation, or none.  state
+    (n_slots, width, channels) of x's type keeps the last inputs (token t at entry t mod width) from call to call: `slots` (B) says which one
+    each sequence owns (default: its own number), `positions` (B) how many tokens it had before (default 0: a new sequence)."""
+    device = x.device
+    code, channels, width = _dtype(x, "x"), x.shape[-1], weight.shape[0]
+    a = _Conv()
+    a.ldx = _matrix(x, "x", device, (channels,))
+    a.weight, a.bias = _vector(weight, "weight", device, (width, channels)), _vector(bias, "bias", device, (channels,))
+    _fill_rows(a.rows, rows, device, x.shape[0], slots, positions, state)
+    if state is not None:
+        a.state = _state(state, "state", device, x.dtype, (width, channels))
+    out = _made(out, x, rows, x.shape)
+    a.ldo = _matrix(out, "out", device, (channels,), x.shape[0])
+    a.x, a.out, a.channels, a.width, a.dtype, a.silu = x.data_ptr(), out.data_ptr(), channels, width, code, bool(silu)
+    _call(_hip.lib().mdf_causal_conv_dev, device, ctypes.byref(a))
+    return out
+
+
+def selective_scan(x, dt, a, b, c, rows: SequenceRows, *, d=None, dt_bias=None, state=None, slots=None, positions=None, out=None):
+    """With D = softplus(dt[t, h] + dt_bias[h]):  H <- exp(D a[h]) H + D x[t, h, :] (x) b[t, g, :],  y[t, h, :] = H c[t, g, :] + d[h] x[t, h, :].
+
+    x and the result (R, heads, head_dim), dt (R, heads), b and c (R, groups, state_dim) -- views into one wider array are fine, only the
+    row strides are free; a, d, dt_bias (heads) f32.  head_dim 1..256, state_dim 1..128, heads a multiple of groups.  state (n_slots, heads,
+    head_dim, state_dim) f32 is continued where positions > 0 and left behind for the next call; slots / positions as in causal_conv."""
+    device = x.device
+    if x.dim() != 3 or b.dim() != 3 or dt.dim() != 2:
+        raise ValueError(f"x, b, dt have {x.dim()}, {b.dim()}, {dt.dim()} dimensions, wanted 3, 3, 2")
+    total, heads, head_dim = x.shape
+    groups, state_dim = b.shape[1:]
+    g = _Scan()
+    g.dtype, g.dt_dtype = _dtype(x, "x"), _dtype(dt, "dt")
+    if b.dtype != x.dtype or c.dtype != x.dtype:
+        raise ValueError(f"x, b, c are {x.dtype}, {b.dtype}, {c.dtype}: one type is wanted")
+    g.ldx, g.lddt = _matrix(x, "x", device, (heads, head_dim)), _matrix(dt, "dt", device, (heads,), total)
+    g.ldb, g.ldc = _matrix(b, "b", device, (groups, state_dim), total), _matrix(c, "c", device, (groups, state_dim), total)
+    g.a, g.d, g.dt_bias = _vector(a, "a", device, (heads,)), _vector(d, "d", device, (heads,)), _vector(dt_bias, "dt_bias", device, (heads,))
+    _fill_rows(g.rows, rows, device, total, slots, positions, state)
+    if state is not None:
+        g.state = _state(state, "state", device, _torch().float32, (heads, head_dim, state_dim))
+    out = _made(out, x, rows, x.shape)
+    g.ldy = _matrix(out, "out", device, (heads, head_dim), total)
+    g.x, g.dt, g.b, g.c, g.y = x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), out.data_ptr()
+    g.heads, g.groups, g.head_dim, g.state_dim = heads, groups, head_dim, state_dim
+    L = _hip.lib()
+    need = L.mdf_scan_workspace_bytes(ctypes.byref(g))
+    work = _torch().empty(need, dtype=_torch().uint8, device=device) if need else None
+    _call(L.mdf_selective_scan_dev, device, ctypes.byref(g), work.data_ptr() if need else None, need)
+    return out
+
+
+def selective_step(xbc, dt, a, *, conv_weight, conv_state, state, positions=None, slots=None, conv_bias=None, d=None, dt_bias=None, out=None):
+    """One token of each of B sequences: causal_conv (silu) of xbc = [x | b | c] (B, heads*head_dim + 2*groups*state_dim), then selective_scan,
+    in one launch; conv_state (n_slots, width, channels) and state (n_slots, heads, head_dim, state_dim) are updated in place.  Returns y
+    (B, heads, head_dim).  The caller adds 1 to the positions of the sequences it continues."""
+    device = xbc.device
+    if state.dim() != 4 or xbc.dim() != 2:
+        raise ValueError(f"state and xbc have {state.dim()}, {xbc.dim()} dimensions, wanted 4, 2")
+    torch = _torch()
+    n, channels = xbc.shape
+    heads, head_dim, state_dim = state.shape[1:]
+    groups, odd = divmod(channels - heads * head_dim, 2 * state_dim) if state_dim else (0, 1)
+    if odd or groups < 1:
+        raise ValueError(f"xbc has {channels} channels: wanted {heads} x {head_dim} and twice a multiple of {state_dim}")
+    width = conv_weight.shape[0]
+    g = _Step()
+    g.dtype, g.dt_dtype = _dtype(xbc, "xbc"), _dtype(dt, "dt")
+    g.ldx, g.lddt = _matrix(xbc, "xbc", device, (channels,)), _matrix(dt, "dt", device, (heads,), n)
+    g.conv_weight, g.conv_bias = _vector(conv_weight, "conv_weight", device, (width, channels)), _vector(conv_bias, "conv_bias", device, (channels,))
+    g.a, g.d, g.dt_bias = _vector(a, "a", device, (heads,)), _vector(d, "d", device, (heads,)), _vector(dt_bias, "dt_bias", device, (heads,))
+    g.conv_state = _state(conv_state, "conv_state", device, xbc.dtype, (width, channels))
+    g.state = _state(state, "state", device, torch.float32, (heads, head_dim, state_dim))
+    if conv_state.shape[0] != state.shape[0]:
+        raise ValueError(f"{conv_state.shape[0]} convolution states beside {state.shape[0]} scan states")
+    g.slots, g.positions = _indices(slots, "slots", device, n), _indices(positions, "positions", device, n)
+    if out is None:
+        out = torch.empty((n, heads, head_dim), dtype=xbc.dtype, device=device) if slots is None else torch.zeros((n, heads, head_dim), dtype=xbc.dtype, device=device)
+    elif out.dtype != xbc.dtype:
+        raise ValueError(f"out is {out.dtype}, the input {xbc.dtype}")
+    g.ldy = _matrix(out, "out", device, (heads, head_dim), n)
+    g.xbc, g.dt, g.y = xbc.data_ptr(), dt.data_ptr(), out.data_ptr()
+    g.B, g.n_slots, g.heads, g.groups, g.head_dim, g.state_dim, g.width = n, state.shape[0], heads, groups, head_dim, state_dim, width
+    _call(_hip.lib().mdf_selective_step_dev, device, ctypes.byref(g))
+    return out
+
+
+def block_norm(s, *, residual=None, gate=None, gate_act: str = "silu", gate_first: bool = False, post_weight=None, post_bias=None, groups: int = 1, scale: float = 1.0,
+               scale_vec=None, pre_weight=None, pre_bias=None, eps: float = 1e-6, center: bool = False, residual_out=None, out=None):
+    """The norms before and after a block with its gate, residual scale and residual, in one pass over the rows of s (rows, dim):
+
+        v = s [* act(gate), with gate_first];  v = post(v) where post_weight is given;  v = v * act(gate) where the gate comes last
+        r = residual + scale * scale_vec * v  where a residual is given;  out = pre(r) where pre_weight is given
+
+    Returns (r or None, out or None); without a residual out is v, or pre(v).  post / pre: x / sqrt(mean(x^2) + eps) * weight + bias, of x less its
+    mean with `center`; post on each of `groups` equal parts of a row.  s and gate share a type; the residual is float32 or of that type, and r has
+    its type.  residual_out may be the residual itself, out may be s or the gate."""
+    device = s.device
+    if s.dim() != 2:
+        raise ValueError(f"s has {s.dim()} dimensions, wanted 2")
+    if gate_act not in ACTS:
+        raise ValueError(f"gate_act {gate_act!r} is none of {sorted(ACTS)}")
+    torch = _torch()
+    rows, dim = s.shape
+    g = _Norm()
+    g.dtype, g.lds, g.s = _dtype(s, "s"), _matrix(s, "s", device, (dim,)), s.data_ptr()
+    if gate is not None:
+        if gate.dtype != s.dtype:
+            raise ValueError(f"gate is {gate.dtype}, s {s.dtype}")
+        g.gate, g.ldg = gate.data_ptr(), _matrix(gate, "gate", device, (dim,), rows)
+    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight), ("pre_bias", pre_bias), ("scale_vec", scale_vec)):
+        if t is not None:
+            setattr(g, name, _vector(t, name, device, (dim,)))
+    if residual is not None:
+        g.residual_dtype, g.residual, g.ldr = _dtype(residual, "residual"), residual.data_ptr(), _matrix(residual, "residual", device, (dim,), rows)
+        if residual_out is None:
+            residual_out = torch.empty((rows, dim), dtype=residual.dtype, device=device)
+        elif residual_out.dtype != residual.dtype:
+            raise ValueError(f"residual_out is {residual_out.dtype}, the residual {residual.dtype}")
+        g.residual_out, g.ldro = residual_out.data_ptr(), _matrix(residual_out, "residual_out", device, (dim,), rows)
+    elif residual_out is not None:
+        raise ValueError("residual_out without a residual")
+    if pre_weight is not None or residual is None:
+        if out is None:
+            out = torch.empty((rows, dim), dtype=s.dtype, device=device)
+        elif out.dtype != s.dtype:
+            raise ValueError(f"out is {out.dtype}, s {s.dtype}")
+        g.out, g.ldo = out.data_ptr(), _matrix(out, "out", device, (dim,), rows)
+    elif out is not None:
+        raise ValueError("out without a pre-norm beside a residual: there is nothing to write there")
+    g.rows, g.dim, g.groups, g.gate_act, g.gate_first, g.center, g.scale, g.eps = rows, dim, groups, ACTS[gate_act], bool(gate_first), bool(center), scale, eps
+    _call(_hip.lib().mdf_block_norm_dev, device, ctypes.byref(g))
+    return residual_out, out

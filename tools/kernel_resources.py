@@ -13,7 +13,7 @@ import tempfile
 ROOT = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..")
 CSRC = os.path.join(ROOT, "metagenomic-deepfri_amd", "csrc")
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-Wno-unused-function"]     # csrc/Makefile: CXXFLAGS
-EXTRA = {"cmap.hip": ["-ffp-contract=off"]}                                                     # csrc/Makefile: the contact kernels' rule
+EXTRA = {"cmap.hip": ["-ffp-contract=off"], "ssm.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}                                                     # csrc/Makefile: the contact kernels' rule
 KEYS = (("VGPRs", r"\bVGPRs: (\d+)"), ("AGPRs", r"\bAGPRs: (\d+)"), ("SGPRs", r"TotalSGPRs: (\d+)"), ("vspill", r"VGPRs Spill: (\d+)"), ("sspill", r"SGPRs Spill: (\d+)"),
         ("scratch", r"ScratchSize \[bytes/lane\]: (\d+)"), ("LDS", r"LDS Size \[bytes/block\]: (\d+)"), ("waves/SIMD", r"Occupancy \[waves/SIMD\]: (\d+)"))
 
