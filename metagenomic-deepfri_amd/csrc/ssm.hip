@@ -2,6 +2,9 @@
 // token, and the norms around the block (include/mdfri.h "Operators of a state-space language-model block").
 #include "common.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace mdf {
 
 typedef unsigned short u16;
@@ -20,13 +23,41 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ Bf16 from_f32<Bf16>(float x) { return {__builtin_bit_cast(u16, (__bf16)x)}; }   // round to nearest even
 template <> __device__ __forceinline__ F16 from_f32<F16>(float x) { return {__builtin_bit_cast(u16, (_Float16)x)}; }
 
-__device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + __expf(-v)); }
+// v_rcp_f32 is within one step: an IEEE division is ten instructions per value, and these run once per element of arrays that stream from memory
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
+__device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
 __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
 // one value of any of the three types, by code (uniform): the step sizes dt, which are read once per head and row
 __device__ __forceinline__ float load_any(const void *p, size_t i, int dt)
 {
     return dt == MDF_DT_F32 ? static_cast<const float *>(p)[i] : dt == MDF_DT_BF16 ? to_f32(static_cast<const Bf16 *>(p)[i]) : to_f32(static_cast<const F16 *>(p)[i]);
+}
+
+// N values as they lie in memory: one 16-byte access (f32: two for 8) at whatever alignment the values themselves have -- the global memory path takes
+// any address, at the price of one more cache line where an access crosses one, so odd strides and views need no code of their own
+template <typename T, int N>
+struct Raw {
+    T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ Raw<T, N> load_raw(const T *p)
+{
+    Raw<T, N> r;
+    __builtin_memcpy(&r, p, sizeof(r));
+    return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_raw(T *p, const Raw<T, N> &r)
+{
+    __builtin_memcpy(p, &r, sizeof(r));
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_f32(T *p, const float *v)
+{
+    Raw<T, N> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(v[i]);
+    store_raw(p, r);
 }
 
 // What a kernel knows of a sequence; count < 0: skipped (its slot is outside the pool, or it has no rows)
@@ -61,38 +92,110 @@ __device__ __forceinline__ int seq_before(const int32_t *row_off, int B, int64_t
     return lo;
 }
 
-// ---- the short causal convolution: simple form, one thread per row and channel ----------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(256) void k_conv_simple(mdf_conv_args g)
+// ---- the short causal convolution ----------------------------------------------------------------------------------------------------------------
+// A thread owns V channels (16 bytes) of `steps` tiles of CONV_ROWS rows.  A tile's rows and the width - 1 in front of them are requested
+// at once (19 loads in flight at width 4), the weights stay in registers over the thread's tiles.  Bound by memory: each element is read and
+// written once, the rows in front of a tile come out of L2.  A tile that lies inside one sequence takes the taps from its registers; one
+// that a sequence begins, ends or skips in goes row by row and looks every tap up (mixed-length batches: a tile or two per sequence).
+// The tile with a sequence's first row makes all of its first width - 1 rows -- the ones that look into the kept state -- wherever they lie, and then
+// keeps the last inputs: nobody else reads or writes these channels' entries, so a short sequence that overwrites an entry it still needed is no race.
+constexpr int CONV_ROWS = 16;
+
+template <typename T, int V, int W>
+__device__ void conv_row(const mdf_conv_args &g, const Seq &s, int t, int c, float (&v)[V])   // one row's sums, every tap looked up
 {
-    const int64_t row = blockIdx.x;
-    const int b = seq_before(g.rows.row_off, g.rows.B, row);
-    if (b < 0) return;
-    const Seq s = seq_of(g.rows, b, g.state != nullptr);
-    const int64_t t = row - s.row;
-    if (t >= s.count) return;
-    const T *x = static_cast<const T *>(g.x);
-    const T *ring = static_cast<const T *>(g.state) + (size_t)s.slot * g.width * g.channels;
-    for (int c = threadIdx.x; c < g.channels; c += 256) {
-        float v = g.bias ? g.bias[c] : 0.0f;
-        for (int k = 0; k < g.width; ++k) {
-            const int back = g.width - 1 - k;
-            float u = 0.0f;
-            if (t >= back) u = to_f32(x[(size_t)(row - back) * g.ldx + c]);
-            else if (g.state && s.pos + t >= back) u = to_f32(ring[(size_t)((s.pos + t - back) % g.width) * g.channels + c]);
-            v = fmaf(g.weight[(size_t)k * g.channels + c], u, v);
-        }
-        static_cast<T *>(g.out)[(size_t)row * g.ldo + c] = from_f32<T>(g.silu ? silu(v) : v);
+    const T *x = static_cast<const T *>(g.x) + (size_t)(s.row + t) * g.ldx + c;
+#pragma unroll
+    for (int back = W - 1; back >= 0; --back) {
+        Raw<T, V> u;
+        if (t >= back) u = load_raw<T, V>(x - (size_t)back * g.ldx);
+        else if (g.state && s.pos + t >= back)
+            u = load_raw<T, V>(static_cast<const T *>(g.state) + ((size_t)s.slot * W + (size_t)((s.pos + t - back) % W)) * g.channels + c);
+        else continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = fmaf(g.weight[(size_t)(W - 1 - back) * g.channels + c + i], to_f32(u.v[i]), v[i]);
     }
 }
-template <typename T>
-__global__ __launch_bounds__(256) void k_conv_ring_simple(mdf_conv_args g)
+
+template <typename T, int V, int W>
+__global__ __launch_bounds__(256) void k_conv(mdf_conv_args g, int steps, int lanes)   // lanes = channels / V, rounded up; channels >= V
 {
-    const Seq s = seq_of(g.rows, blockIdx.x, true);
-    T *ring = static_cast<T *>(g.state) + (size_t)s.slot * g.width * g.channels;
-    for (int t = max(0, s.count - g.width); t < s.count; ++t)
-        for (int c = threadIdx.x; c < g.channels; c += 256)
-            ring[(size_t)((s.pos + t) % g.width) * g.channels + c] = static_cast<const T *>(g.x)[(size_t)(s.row + t) * g.ldx + c];
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t tile0 = id / lanes * steps;
+    // The last lane of an uneven row is moved up against the row's end: it makes `twice` channels that its neighbour makes too, to the same bits -- but
+    // for a sequence's first rows, whose kept inputs the neighbour may have replaced already, it stores its own channels only.
+    const int c = min((int)(id % lanes) * V, g.channels - V), twice = (int)(id % lanes) * V - c;
+    if (tile0 * CONV_ROWS >= g.rows.R) return;
+    Raw<float, V> w[W], bias = {};
+#pragma unroll
+    for (int k = 0; k < W; ++k) w[k] = load_raw<float, V>(g.weight + (size_t)k * g.channels + c);
+    if (g.bias) bias = load_raw<float, V>(g.bias + c);
+    int b = seq_before(g.rows.row_off, g.rows.B, tile0 * CONV_ROWS);
+    for (int step = 0; step < steps; ++step) {
+        const int64_t r0 = (tile0 + step) * CONV_ROWS, r1 = min(r0 + CONV_ROWS, g.rows.R);
+        if (r0 >= r1) return;
+        while (b + 1 < g.rows.B && g.rows.row_off[b + 1] <= r0) ++b;
+        Seq s = {0, -1, 0, 0};
+        if (b >= 0) s = seq_of(g.rows, b, g.state != nullptr);
+        if (s.count > 0 && r0 - s.row >= max(W - 1, 1) && r1 - s.row <= s.count && r1 - r0 == CONV_ROWS) {
+            Raw<T, V> raw[CONV_ROWS + W - 1];
+            const T *x = static_cast<const T *>(g.x) + (size_t)(r0 - (W - 1)) * g.ldx + c;
+#pragma unroll
+            for (int k = 0; k < CONV_ROWS + W - 1; ++k) raw[k] = load_raw<T, V>(x + (size_t)k * g.ldx);
+            T *out = static_cast<T *>(g.out) + (size_t)r0 * g.ldo + c;
+#pragma unroll
+            for (int r = 0; r < CONV_ROWS; ++r) {
+                float v[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    v[i] = bias.v[i];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) v[i] = fmaf(w[k].v[i], to_f32(raw[r + k].v[i]), v[i]);
+                    if (g.silu) v[i] = silu(v[i]);
+                }
+                store_f32<T, V>(out + (size_t)r * g.ldo, v);
+            }
+            continue;
+        }
+        auto row = [&](int t) {
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = bias.v[i];
+            conv_row<T, V, W>(g, s, t, c, v);
+            if (g.silu)
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = silu(v[i]);
+            T *out = static_cast<T *>(g.out) + (size_t)(s.row + t) * g.ldo + c;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i >= twice) out[i] = from_f32<T>(v[i]);
+        };
+        auto keep = [&]() {   // the sequence's last W inputs into its state
+            if (!g.state) return;
+            for (int t = max(0, s.count - W); t < s.count; ++t) {
+                const Raw<T, V> last = load_raw<T, V>(static_cast<const T *>(g.x) + (size_t)(s.row + t) * g.ldx + c);
+                T *entry = static_cast<T *>(g.state) + ((size_t)s.slot * W + (size_t)((s.pos + t) % W)) * g.channels + c;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (i >= twice) entry[i] = last.v[i];
+            }
+        };
+        bool began = b >= 0 && s.row >= r0;
+        for (int64_t r = r0; r < r1; ++r) {
+            while (b + 1 < g.rows.B && g.rows.row_off[b + 1] <= r) {
+                if (began) keep();
+                s = seq_of(g.rows, ++b, g.state != nullptr);
+                began = true;
+            }
+            const int64_t t = r - s.row;
+            if (b < 0 || t >= s.count || (!began && t < W - 1)) continue;
+            row((int)t);
+        }
+        if (began) {
+            for (int t = (int)(r1 - s.row); t < min(s.count, W - 1); ++t) row(t);
+            keep();
+        }
+    }
 }
 
 // ---- the selective scan: simple form, one workgroup per sequence, head and 64 channels, the state in LDS ---------------------------------
@@ -131,42 +234,209 @@ __global__ __launch_bounds__(64) void k_scan_simple(mdf_scan_args g)
         for (int n = 0; n < N; ++n) st[n] = H[threadIdx.x][n];
 }
 
-// ---- one token: simple form, one workgroup per sequence and head ---------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(256) void k_step_simple(mdf_step_args g)
+// ---- one token of many sequences -----------------------------------------------------------------------------------------------------------------------
+// Bound by the states' traffic, 8 bytes per state element; for a few sequences by latency.  A workgroup owns `rows` channels of one head: LN lanes hold a
+// channel's state_dim values (V each, J times), 256 / LN channels go at once.  All its state is requested first, then the convolution of its own
+// channels and of the group's B and C is made into LDS (every workgroup of a group makes B and C again: 2 N width products against a state of
+// rows x N), then the state is advanced in registers and stored where it came from.
+// The convolution's state is a ring: this token's entry, pos mod width, is the one entry no workgroup reads, so each input is stored by one
+// workgroup at once without waiting for the others.
+template <typename T, int LN, int V, int J>
+__global__ __launch_bounds__(256) void k_step(mdf_step_args g, int rows)
 {
-    __shared__ float u[256 + 2 * 128];   // the head's x, B, C after the convolution
-    const int b = blockIdx.x, h = blockIdx.y, r = g.heads / g.groups, grp = h / r, P = g.head_dim, N = g.state_dim, W = g.width;
+    constexpr int PER = 256 / LN, MOST = 8;   // channels at once; the most a thread holds
+    __shared__ float u[PER * MOST + 2 * 128];
+    const int b = blockIdx.x, h = blockIdx.y, p0 = blockIdx.z * rows, r = g.heads / g.groups, grp = h / r, P = g.head_dim, N = g.state_dim, W = g.width;
     const int slot = g.slots ? g.slots[b] : b;
     if (slot < 0 || slot >= g.n_slots) return;
-    const int64_t pos = g.positions ? max(g.positions[b], 0) : 0;
-    const int channels = g.heads * P + 2 * g.groups * N;
+    const unsigned pos = g.positions ? (unsigned)max(g.positions[b], 0) : 0u;
+    const int channels = g.heads * P + 2 * g.groups * N, count = min(rows, P - p0);
+    const int lane = threadIdx.x % LN, sub = threadIdx.x / LN;
+    float *state = g.state + (((size_t)slot * g.heads + h) * P + p0) * N;
+    Raw<float, V> st[MOST][J];
+#pragma unroll
+    for (int k = 0; k < MOST; ++k)
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int p = k * PER + sub, n = (j * LN + lane) * V;
+            st[k][j] = {};
+            if (p < count && n < N && pos > 0) st[k][j] = load_raw<float, V>(state + (size_t)p * N + n);
+        }
     T *ring = static_cast<T *>(g.conv_state) + (size_t)slot * W * channels;
-    for (int i = threadIdx.x; i < P + 2 * N; i += 256) {
-        const int c = i < P ? h * P + i : i < P + N ? g.heads * P + grp * N + i - P : g.heads * P + (g.groups + grp) * N + i - P - N;
+    for (int i = threadIdx.x; i < count + 2 * N; i += 256) {
+        const int c = i < count ? h * P + p0 + i : g.heads * P + (i < count + N ? grp * N + i - count : (g.groups + grp) * N + i - count - N);
         const T now = static_cast<const T *>(g.xbc)[(size_t)b * g.ldx + c];
         float v = g.conv_bias ? g.conv_bias[c] : 0.0f;
-        for (int back = W - 1; back > 0; --back)
+#pragma unroll 4
+        for (unsigned back = W - 1; back > 0; --back)
             if (pos >= back) v = fmaf(g.conv_weight[(size_t)(W - 1 - back) * channels + c], to_f32(ring[(size_t)((pos - back) % W) * channels + c]), v);
         v = fmaf(g.conv_weight[(size_t)(W - 1) * channels + c], to_f32(now), v);
-        u[i] = silu(v);
-        if (i < P || h % r == 0) ring[(size_t)(pos % W) * channels + c] = now;   // an entry that no workgroup of this launch reads
+        u[i < count ? i : i - count + PER * MOST] = silu(v);
+        if (i < count || (h % r == 0 && p0 == 0)) ring[(size_t)(pos % W) * channels + c] = now;
     }
-    __syncthreads();
     const float delta = softplus(load_any(g.dt, (size_t)b * g.lddt + h, g.dt_dtype) + (g.dt_bias ? g.dt_bias[h] : 0.0f)), decay = expf(delta * g.a[h]);
-    for (int p = threadIdx.x; p < P; p += 256) {
-        float *st = g.state + (((size_t)slot * g.heads + h) * P + p) * N;
-        float y = g.d ? g.d[h] * u[p] : 0.0f;
-        for (int n = 0; n < N; ++n) {
-            const float v = fmaf(decay, pos > 0 ? st[n] : 0.0f, delta * u[p] * u[P + n]);
-            st[n] = v;
-            y = fmaf(v, u[P + N + n], y);
+    const float skip = g.d ? g.d[h] : 0.0f;
+    __syncthreads();
+    float B[J][V], C[J][V];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int n = (j * LN + lane) * V + i;
+            B[j][i] = n < N ? u[PER * MOST + n] : 0.0f;
+            C[j][i] = n < N ? u[PER * MOST + N + n] : 0.0f;
         }
-        static_cast<T *>(g.y)[(size_t)b * g.ldy + (size_t)h * P + p] = from_f32<T>(y);
+#pragma unroll
+    for (int k = 0; k < MOST; ++k) {
+        const int p = k * PER + sub;
+        if (k * PER >= count) break;
+        const float x = p < count ? u[p] : 0.0f, dx = delta * x;
+        float y = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int n = (j * LN + lane) * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                st[k][j].v[i] = fmaf(decay, st[k][j].v[i], dx * B[j][i]);
+                y = fmaf(st[k][j].v[i], C[j][i], y);
+            }
+            if (p < count && n < N) store_raw(state + (size_t)p * N + n, st[k][j]);
+        }
+#pragma unroll
+        for (int m = 1; m < LN; m <<= 1) y += __shfl_xor(y, m);
+        if (lane == 0 && p < count) static_cast<T *>(g.y)[(size_t)b * g.ldy + (size_t)h * P + p0 + p] = from_f32<T>(g.d ? fmaf(skip, x, y) : y);
     }
 }
 
-// ---- block norms: simple form, one workgroup per row and group, three walks over the row ------------------------------------------------------
+// ---- block norms ------------------------------------------------------------------------------------------------------------------------------------
+// One pass: a row's inputs are requested together, live in registers as f32 through both norms and leave once.  TPR threads per (row, group) hold
+// VPT x 8 values each: a wave holds widths to 2 048 (its sums need no LDS), 256 threads to 8 192, 1 024 to 16 384.  Bound by memory.  Sums: in order
+// over a thread's values, then a tree over lanes -- the same for every row, whatever the batch.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float *part)
+{
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+    if constexpr (TPR > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) v += part[i];
+    }
+    return v;
+}
+
+// thread t of a row holds the 8 values from (v TPR + t) 8 on; a row's last few are taken one by one
+template <typename T, typename R, int TPR, int VPT>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_block_norm(mdf_block_norm_args g)
+{
+    __shared__ float part[16];
+    const int t = threadIdx.x % TPR, width = g.dim / g.groups, c0 = blockIdx.y * width;
+    const size_t row = TPR < 256 ? (size_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : blockIdx.x;
+    if (row >= (size_t)g.rows) return;    // whole waves (TPR = 64) only
+    const T *s = static_cast<const T *>(g.s) + row * g.lds + c0, *gate = static_cast<const T *>(g.gate) + row * g.ldg + c0;
+    const R *res = static_cast<const R *>(g.residual) + row * g.ldr + c0;
+    auto left = [&](int v) { return width - (v * TPR + t) * 8; };   // values from vector v's first to the row's end
+    auto load = [&](auto *p, auto &raw, int v) {
+        const int n = left(v);
+        p += (v * TPR + t) * 8;
+        raw = {};
+        if (n >= 8) raw = load_raw<typename std::remove_const<typename std::remove_pointer<decltype(p)>::type>::type, 8>(p);
+        else if (n > 0)
+#pragma unroll
+            for (int e = 0; e < 7; ++e)
+                if (e < n) raw.v[e] = p[e];
+    };
+    auto param = [&](const float *p, int v) {   // 8 parameters of vector v
+        Raw<float, 8> r;
+        load(p + c0, r, v);
+        return r;
+    };
+    Raw<T, 8> rs[VPT], rg[VPT];
+    Raw<R, 8> rr[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) load(s, rs[v], v);
+    if (g.gate)
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) load(gate, rg[v], v);
+    if (g.residual)
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) load(res, rr[v], v);
+    float x[VPT][8];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[v][e] = to_f32(rs[v].v[e]);
+    auto gated = [&]() {
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float z = to_f32(rg[v].v[e]);
+                x[v][e] *= g.gate_act == MDF_ACT_SILU ? silu(z) : g.gate_act == MDF_ACT_SIGMOID ? sigmoid(z) : z;
+            }
+        }
+    };
+    // values beyond the row are zeros going in; the centred sum of squares leaves them out again
+    auto norm = [&](const float *weight, const float *bias) {
+        const float inv = 1.0f / (float)width;
+        float mean = 0.0f, sum = 0.0f;
+        if (g.center) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mean += x[v][e];
+            mean = row_sum<TPR>(mean, part) * inv;
+        }
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (e < left(v)) x[v][e] -= mean;
+                sum = fmaf(x[v][e], x[v][e], sum);
+            }
+        const float q = 1.0f / sqrtf(row_sum<TPR>(sum, part) * inv + g.eps);
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            Raw<float, 8> w = param(weight, v), o = {};
+            if (bias) o = param(bias, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[v][e] = fmaf(x[v][e] * q, w.v[e], o.v[e]);
+        }
+    };
+    auto store = [&](auto *p) {
+        typedef typename std::remove_pointer<decltype(p)>::type O;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int n = left(v);
+            O *q = p + (v * TPR + t) * 8;
+            if (n >= 8) store_f32<O, 8>(q, x[v]);
+            else if (n > 0)
+#pragma unroll
+                for (int e = 0; e < 7; ++e)
+                    if (e < n) q[e] = from_f32<O>(x[v][e]);
+        }
+    };
+    if (g.gate && g.gate_first) gated();
+    if (g.post_weight) norm(g.post_weight, g.post_bias);
+    if (g.gate && !g.gate_first) gated();
+    if (g.residual) {
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            Raw<float, 8> k = {};
+            if (g.scale_vec) k = param(g.scale_vec, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[v][e] = fmaf(g.scale_vec ? g.scale * k.v[e] : g.scale, x[v][e], to_f32(rr[v].v[e]));
+        }
+        store(static_cast<R *>(g.residual_out) + row * g.ldro + c0);
+    }
+    if (g.pre_weight) norm(g.pre_weight, g.pre_bias);
+    if (g.out) store(static_cast<T *>(g.out) + row * g.ldo + c0);
+}
+
+// Rows wider than the registers of 1 024 threads hold (16 384 values): one workgroup walks the row three times, the second and third out of L2
 __device__ __forceinline__ float block_sum(float v)
 {
     __shared__ float part[4];
@@ -177,7 +447,7 @@ __device__ __forceinline__ float block_sum(float v)
     return (part[0] + part[1]) + (part[2] + part[3]);
 }
 template <typename T, typename R>
-__global__ __launch_bounds__(256) void k_block_norm_simple(mdf_block_norm_args g)
+__global__ __launch_bounds__(256) void k_block_norm_walk(mdf_block_norm_args g)
 {
     const size_t row = blockIdx.x;
     const int width = g.dim / g.groups, c0 = blockIdx.y * width, c1 = c0 + width;
@@ -241,6 +511,60 @@ static bool overlap(const void *p, int64_t ldp, int64_t wp, size_t ep, const voi
     return true;
 }
 
+template <typename T, typename R, int TPR, int VPT>
+static void norm_launch(const mdf_block_norm_args &a, hipStream_t st)
+{
+    const dim3 grid((unsigned)(TPR < 256 ? (a.rows + 256 / TPR - 1) / (256 / TPR) : a.rows), a.groups), block(TPR < 256 ? 256 : TPR);
+    hipLaunchKernelGGL((k_block_norm<T, R, TPR, VPT>), grid, block, 0, st, a);
+}
+template <typename T, typename R>
+static void norm_by_width(const mdf_block_norm_args &a, hipStream_t st)
+{
+    const int width = a.dim / a.groups;
+    if (width <= 512) norm_launch<T, R, 64, 1>(a, st);
+    else if (width <= 1024) norm_launch<T, R, 64, 2>(a, st);
+    else if (width <= 2048) norm_launch<T, R, 64, 4>(a, st);
+    else if (width <= 4096) norm_launch<T, R, 256, 2>(a, st);
+    else if (width <= 8192) norm_launch<T, R, 256, 4>(a, st);
+    else if (width <= 16384) norm_launch<T, R, 1024, 2>(a, st);
+    else hipLaunchKernelGGL((k_block_norm_walk<T, R>), dim3((unsigned)a.rows, a.groups), dim3(256), 0, st, a);
+}
+
+template <typename T>
+static void step_launch(const mdf_step_args &a, hipStream_t st)
+{
+    const int N = a.state_dim;
+    const bool wide = N % 4 == 0;   // else one value at a time
+    const int ln = wide ? (N <= 16 ? 4 : N <= 32 ? 8 : N <= 64 ? 16 : 32) : N <= 16 ? 16 : N <= 32 ? 32 : 64;
+    const int per = 256 / ln;
+    // channels per workgroup: as many as a thread's registers hold (8 x `per`) while that leaves four workgroups per CU, fewer for few sequences
+    int rows = std::min(a.head_dim, 8 * per);
+    while (rows > per && (int64_t)a.B * a.heads * ((a.head_dim + rows - 1) / rows) < 1024) rows = std::max(per, (rows / 2 + per - 1) / per * per);
+    const dim3 grid((unsigned)a.B, a.heads, (a.head_dim + rows - 1) / rows);
+#define MDF_S(ln_, v_, j_) hipLaunchKernelGGL((k_step<T, ln_, v_, j_>), grid, dim3(256), 0, st, a, rows)
+    if (wide) {
+        if (ln == 4) MDF_S(4, 4, 1);
+        else if (ln == 8) MDF_S(8, 4, 1);
+        else if (ln == 16) MDF_S(16, 4, 1);
+        else MDF_S(32, 4, 1);
+    } else {
+        if (ln == 16) MDF_S(16, 1, 1);
+        else if (ln == 32) MDF_S(32, 1, 1);
+        else MDF_S(64, 1, 2);
+    }
+#undef MDF_S
+}
+
+template <typename T, int V>
+static void conv_launch(const mdf_conv_args &a, int steps, int lanes, dim3 grid, hipStream_t st)
+{
+    switch (a.width) {
+#define MDF_W(w_) case w_: hipLaunchKernelGGL((k_conv<T, V, w_>), grid, dim3(256), 0, st, a, steps, lanes); break;
+        MDF_W(1) MDF_W(2) MDF_W(3) MDF_W(4) MDF_W(5) MDF_W(6) MDF_W(7) MDF_W(8)
+#undef MDF_W
+    }
+}
+
 static int check_rows(const mdf_seq_rows &r, const char *who, bool kept)
 {
     MDF_REQUIRE(r.B >= 0 && r.R >= 0 && r.R < (int64_t)1 << 31, "%s: B=%d sequences, R=%lld rows", who, r.B, (long long)r.R);
@@ -276,9 +600,18 @@ int mdf_causal_conv_dev(const mdf_conv_args *a, void *stream)
     MDF_REQUIRE(!overlap(a->x, a->ldx, a->channels, e, a->out, a->ldo, a->channels, e, a->rows.R), "causal_conv_dev: out overlaps x");
     if (int rc = require_device()) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
+    const int v = a->channels >= 16 / (int)e ? 16 / (int)e : 1;
+    const int lanes = (a->channels + v - 1) / v;
+    // tiles per thread: the weights cost 4 (width + 1) bytes per channel and thread, so as many as leave the GPU 4 waves per SIMD to run (256 x 4 x 4)
+    const int64_t tiles = (a->rows.R + CONV_ROWS - 1) / CONV_ROWS;
+    int steps = 1;
+    while (steps < 4 && tiles * lanes >= (int64_t)2 * steps * 64 * 4096) steps *= 2;
+    const int64_t threads = (tiles + steps - 1) / steps * lanes;
+    MDF_REQUIRE((threads + 255) / 256 < (int64_t)1 << 31, "causal_conv_dev: %lld rows of %d channels are too many", (long long)a->rows.R, a->channels);
+    const dim3 grid((unsigned)((threads + 255) / 256));
     MDF_BY_TYPE(a->dtype, T, {
-        hipLaunchKernelGGL(k_conv_simple<T>, dim3((unsigned)a->rows.R), dim3(256), 0, st, *a);
-        if (a->state) hipLaunchKernelGGL(k_conv_ring_simple<T>, dim3((unsigned)a->rows.B), dim3(256), 0, st, *a);
+        if (v > 1) conv_launch<T, 16 / sizeof(T)>(*a, steps, lanes, grid, st);
+        else conv_launch<T, 1>(*a, steps, lanes, grid, st);
     });
     MDF_HIP(hipGetLastError());
     return MDF_OK;
@@ -329,7 +662,7 @@ int mdf_selective_step_dev(const mdf_step_args *a, void *stream)
                 "selective_step_dev: y overlaps an input");
     if (int rc = require_device()) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    MDF_BY_TYPE(a->dtype, T, hipLaunchKernelGGL(k_step_simple<T>, dim3(a->B, a->heads), dim3(256), 0, st, *a));
+    MDF_BY_TYPE(a->dtype, T, step_launch<T>(*a, st));
     MDF_HIP(hipGetLastError());
     return MDF_OK;
 }
@@ -363,9 +696,11 @@ int mdf_block_norm_dev(const mdf_block_norm_args *a, void *stream)
     MDF_REQUIRE(!overlap(out[0].p, out[0].ld, d, er, out[1].p, out[1].ld, d, e, a->rows), "block_norm_dev: the outputs overlap");
     if (int rc = require_device()) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
+    mdf_block_norm_args k = *a;
+    if (!has_out) k.out = nullptr;
     MDF_BY_TYPE(a->dtype, T, {
-        if (a->residual && a->residual_dtype == MDF_DT_F32) hipLaunchKernelGGL((k_block_norm_simple<T, float>), dim3((unsigned)a->rows, a->groups), dim3(256), 0, st, *a);
-        else hipLaunchKernelGGL((k_block_norm_simple<T, T>), dim3((unsigned)a->rows, a->groups), dim3(256), 0, st, *a);
+        if (a->residual && a->residual_dtype == MDF_DT_F32) norm_by_width<T, float>(k, st);
+        else norm_by_width<T, T>(k, st);
     });
     MDF_HIP(hipGetLastError());
     return MDF_OK;
