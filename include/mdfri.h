@@ -299,6 +299,7 @@ typedef struct {
     void *y;
     int64_t ldx, lddt, ldy;
     int32_t B, n_slots, heads, groups, head_dim, state_dim, width, dtype, dt_dtype;
+    int32_t zero_skipped;   /* y of a skipped sequence: zeros (1), or left as it is (0) */
 } mdf_step_args;
 int mdf_selective_step_dev(const mdf_step_args *args, void *stream);
 

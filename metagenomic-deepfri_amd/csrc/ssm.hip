@@ -55,8 +55,17 @@ template <typename T, int N>
 __device__ __forceinline__ void store_f32(T *p, const float *v)
 {
     Raw<T, N> r;
+    if constexpr (std::is_same<T, Bf16>::value && N % 2 == 0) {   // one conversion for two values
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        unsigned u[N / 2];
 #pragma unroll
-    for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(v[i]);
+        for (int i = 0; i < N; i += 2) u[i / 2] = __builtin_bit_cast(unsigned, __builtin_convertvector((f2){v[i], v[i + 1]}, b2));
+        __builtin_memcpy(&r, u, sizeof(r));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.v[i] = from_f32<T>(v[i]);
+    }
     store_raw(p, r);
 }
 
@@ -93,32 +102,15 @@ __device__ __forceinline__ int seq_before(const int32_t *row_off, int B, int64_t
 }
 
 // ---- the short causal convolution ----------------------------------------------------------------------------------------------------------------
-// A thread owns V channels (16 bytes) of `steps` tiles of CONV_ROWS rows.  A tile's rows and the width - 1 in front of them are requested
-// at once (19 loads in flight at width 4), the weights stay in registers over the thread's tiles.  Bound by memory: each element is read and
-// written once, the rows in front of a tile come out of L2.  A tile that lies inside one sequence takes the taps from its registers; one
-// that a sequence begins, ends or skips in goes row by row and looks every tap up (mixed-length batches: a tile or two per sequence).
-// The tile with a sequence's first row makes all of its first width - 1 rows -- the ones that look into the kept state -- wherever they lie, and then
-// keeps the last inputs: nobody else reads or writes these channels' entries, so a short sequence that overwrites an entry it still needed is no race.
-constexpr int CONV_ROWS = 16;
+// A thread owns V channels (16 bytes) of `steps` tiles of CONV_ROWS rows.  A tile's rows are requested at once, the width - 1 in front of them are still
+// in registers from the tile before (or requested too), the weights stay in registers.  Bound by memory: each element is read and written once.
+// Rows take their taps from registers; only a sequence's first width - 1 rows, which look into the kept state or before the sequence, look
+// every tap up.  The tile with a sequence's first row makes all of those rows, wherever they lie, and then keeps the sequence's last inputs:
+// nobody else reads or writes these channels' entries, so a short sequence that overwrites an entry it still needed is no race.
+constexpr int CONV_ROWS = 8;
 
 template <typename T, int V, int W>
-__device__ void conv_row(const mdf_conv_args &g, const Seq &s, int t, int c, float (&v)[V])   // one row's sums, every tap looked up
-{
-    const T *x = static_cast<const T *>(g.x) + (size_t)(s.row + t) * g.ldx + c;
-#pragma unroll
-    for (int back = W - 1; back >= 0; --back) {
-        Raw<T, V> u;
-        if (t >= back) u = load_raw<T, V>(x - (size_t)back * g.ldx);
-        else if (g.state && s.pos + t >= back)
-            u = load_raw<T, V>(static_cast<const T *>(g.state) + ((size_t)s.slot * W + (size_t)((s.pos + t - back) % W)) * g.channels + c);
-        else continue;
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = fmaf(g.weight[(size_t)(W - 1 - back) * g.channels + c + i], to_f32(u.v[i]), v[i]);
-    }
-}
-
-template <typename T, int V, int W>
-__global__ __launch_bounds__(256) void k_conv(mdf_conv_args g, int steps, int lanes)   // lanes = channels / V, rounded up; channels >= V
+__global__ __launch_bounds__(256, W <= 3 ? 3 : 2) void k_conv(mdf_conv_args g, int steps, int lanes)   // lanes = channels / V, rounded up; channels >= V
 {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t tile0 = id / lanes * steps;
@@ -130,108 +122,447 @@ __global__ __launch_bounds__(256) void k_conv(mdf_conv_args g, int steps, int la
 #pragma unroll
     for (int k = 0; k < W; ++k) w[k] = load_raw<float, V>(g.weight + (size_t)k * g.channels + c);
     if (g.bias) bias = load_raw<float, V>(g.bias + c);
+    const T *x = static_cast<const T *>(g.x) + c;
+    T *out = static_cast<T *>(g.out) + c, *ring = static_cast<T *>(g.state) + c;
     int b = seq_before(g.rows.row_off, g.rows.B, tile0 * CONV_ROWS);
+    Seq s = {0, -1, 0, 0};
+    int64_t next;   // first row of the sequence behind s
+    auto begin = [&]() {
+        if (b >= 0) s = seq_of(g.rows, b, g.state != nullptr);
+        next = b + 1 < g.rows.B ? g.rows.row_off[b + 1] : g.rows.R;
+    };
+    begin();
+    Raw<T, V> raw[CONV_ROWS + W - 1];
     for (int step = 0; step < steps; ++step) {
         const int64_t r0 = (tile0 + step) * CONV_ROWS, r1 = min(r0 + CONV_ROWS, g.rows.R);
         if (r0 >= r1) return;
-        while (b + 1 < g.rows.B && g.rows.row_off[b + 1] <= r0) ++b;
-        Seq s = {0, -1, 0, 0};
-        if (b >= 0) s = seq_of(g.rows, b, g.state != nullptr);
-        if (s.count > 0 && r0 - s.row >= max(W - 1, 1) && r1 - s.row <= s.count && r1 - r0 == CONV_ROWS) {
-            Raw<T, V> raw[CONV_ROWS + W - 1];
-            const T *x = static_cast<const T *>(g.x) + (size_t)(r0 - (W - 1)) * g.ldx + c;
-#pragma unroll
-            for (int k = 0; k < CONV_ROWS + W - 1; ++k) raw[k] = load_raw<T, V>(x + (size_t)k * g.ldx);
-            T *out = static_cast<T *>(g.out) + (size_t)r0 * g.ldo + c;
-#pragma unroll
-            for (int r = 0; r < CONV_ROWS; ++r) {
+        unsigned mask = (1u << CONV_ROWS) - 1;   // rows whose taps are all in registers
+        if (!(r0 - s.row >= max(W - 1, 1) && r0 + CONV_ROWS - s.row <= s.count)) {   // (the next sequence begins behind this one's rows)
+            auto row = [&](int t) {   // one of a sequence's first rows
                 float v[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    v[i] = bias.v[i];
+                for (int i = 0; i < V; ++i) v[i] = bias.v[i];
 #pragma unroll
-                    for (int k = 0; k < W; ++k) v[i] = fmaf(w[k].v[i], to_f32(raw[r + k].v[i]), v[i]);
-                    if (g.silu) v[i] = silu(v[i]);
+                for (int back = W - 1; back >= 0; --back) {
+                    Raw<T, V> u = {};
+                    if (t >= back) u = load_raw<T, V>(x + (size_t)(s.row + t - back) * g.ldx);
+                    else if (g.state && s.pos + t >= back) u = load_raw<T, V>(ring + ((size_t)s.slot * W + (size_t)((s.pos + t - back) % W)) * g.channels);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[i] = fmaf(w[W - 1 - back].v[i], to_f32(u.v[i]), v[i]);
                 }
-                store_f32<T, V>(out + (size_t)r * g.ldo, v);
-            }
-            continue;
-        }
-        auto row = [&](int t) {
-            float v[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = bias.v[i];
-            conv_row<T, V, W>(g, s, t, c, v);
-            if (g.silu)
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = silu(v[i]);
-            T *out = static_cast<T *>(g.out) + (size_t)(s.row + t) * g.ldo + c;
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i >= twice) out[i] = from_f32<T>(v[i]);
-        };
-        auto keep = [&]() {   // the sequence's last W inputs into its state
-            if (!g.state) return;
-            for (int t = max(0, s.count - W); t < s.count; ++t) {
-                const Raw<T, V> last = load_raw<T, V>(static_cast<const T *>(g.x) + (size_t)(s.row + t) * g.ldx + c);
-                T *entry = static_cast<T *>(g.state) + ((size_t)s.slot * W + (size_t)((s.pos + t) % W)) * g.channels + c;
+                T *o = out + (size_t)(s.row + t) * g.ldo;
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    if (i >= twice) entry[i] = last.v[i];
+                    if (i >= twice) o[i] = from_f32<T>(g.silu ? silu(v[i]) : v[i]);
+            };
+            auto finish = [&](int from) {   // the first rows from `from` on, then the sequence's last inputs into its state
+                for (int t = from; t < min(s.count, W - 1); ++t) row(t);
+                if (!g.state) return;
+                Raw<T, V> last[W];
+#pragma unroll
+                for (int k = 0; k < W; ++k) last[k] = load_raw<T, V>(x + (size_t)(s.row + max(s.count - W + k, 0)) * g.ldx);
+#pragma unroll
+                for (int k = 0; k < W; ++k)
+                    if (s.count - W + k >= 0) {
+                        T *entry = ring + ((size_t)s.slot * W + (size_t)((s.pos + s.count - W + k) % W)) * g.channels;
+#pragma unroll
+                        for (int i = 0; i < V; ++i)
+                            if (i >= twice) entry[i] = last[k].v[i];
+                    }
+            };
+            mask = 0;
+            for (int64_t r = r0; r < r1; ++r) {
+                while (r >= next) ++b, begin();
+                const int64_t t = r - s.row;
+                if (b < 0 || t >= s.count) continue;
+                if (t == 0) finish(0);
+                if (t >= W - 1) mask |= 1u << (int)(r - r0);
             }
-        };
-        bool began = b >= 0 && s.row >= r0;
-        for (int64_t r = r0; r < r1; ++r) {
-            while (b + 1 < g.rows.B && g.rows.row_off[b + 1] <= r) {
-                if (began) keep();
-                s = seq_of(g.rows, ++b, g.state != nullptr);
-                began = true;
-            }
-            const int64_t t = r - s.row;
-            if (b < 0 || t >= s.count || (!began && t < W - 1)) continue;
-            row((int)t);
         }
-        if (began) {
-            for (int t = (int)(r1 - s.row); t < min(s.count, W - 1); ++t) row(t);
-            keep();
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) raw[k] = step ? raw[CONV_ROWS + k] : load_raw<T, V>(x + (size_t)max(r0 - (W - 1) + k, (int64_t)0) * g.ldx);
+#pragma unroll
+        for (int k = 0; k < CONV_ROWS; ++k) raw[W - 1 + k] = load_raw<T, V>(x + (size_t)min(r0 + k, g.rows.R - 1) * g.ldx);
+        auto make = [&](int r) {
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[i] = bias.v[i];
+#pragma unroll
+                for (int k = 0; k < W; ++k) v[i] = fmaf(w[k].v[i], to_f32(raw[r + k].v[i]), v[i]);
+                if (g.silu) v[i] = silu(v[i]);
+            }
+            store_f32<T, V>(out + (size_t)(r0 + r) * g.ldo, v);
+        };
+        if (mask == (1u << CONV_ROWS) - 1) {
+#pragma unroll
+            for (int r = 0; r < CONV_ROWS; ++r) make(r);
+        } else {
+#pragma unroll
+            for (int r = 0; r < CONV_ROWS; ++r)
+                if (mask >> r & 1) make(r);
         }
     }
 }
 
-// ---- the selective scan: simple form, one workgroup per sequence, head and 64 channels, the state in LDS ---------------------------------
-template <typename T>
-__global__ __launch_bounds__(64) void k_scan_simple(mdf_scan_args g)
+// ---- the selective scan ----------------------------------------------------------------------------------------------------------------------------
+// Chunks of 32 rows.  With c_i the running log-decay inside a chunk (c_i <= 0, base 2), S the state in front of it and D_j the step sizes, the recurrence is
+//     Y = diag(2^c_i) (C S)  +  M X + d X,      M_ij = (C_i . B_j) 2^(c_i - c_j) D_j  for j <= i, 0 above
+//     S <- 2^c_31 S + B^T diag(D_j 2^(c_31 - c_j)) X
+// -- four products on the bf16 matrix instruction (32 x 32 x 16), all sums and the state in f32.  A wave owns 32 channels of a head and their whole
+// state (16 registers per 32 state values); four waves of a workgroup, channels of the same group of heads, share the chunk's B and C in LDS.
+// No operand goes through LDS on its way from one product to the next: the state comes out of its product with four consecutive n per lane in the very
+// place where the next product takes them as its k, and (B C^T) comes out transposed so that M's rows lie along lanes; the k order of those products is
+// therefore 0-3, 8-11 | 4-7, 12-15 per 16, and B, C are laid into LDS in that order (bits 2 and 3 of the index exchanged).
+// Operands are sums of bfloat16 terms: bfloat16 inputs are one, float16 two and float32 three (all exact).  M and S, which only feed rounded outputs, take two
+// terms (2^-17) for the 16-bit types and three for float32; what goes into the state takes three always, so the state is a float32 one for every type.
+// Bound for bfloat16 by issue: per chunk and wave 52 matrix instructions (state_dim 128) and about twice their time of vector instructions.
+// Long sequences are cut into segments when there are too few (sequence, head) pairs to fill the GPU: a first launch makes each segment's state from zero
+// (STATE: no Y, no C), a small one carries the states from segment to segment, the last one makes Y.
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ unsigned cvt_pk_bf16(float a, float b)
 {
-    __shared__ float H[64][129];
-    __shared__ float B[128], C[128];
-    const int h = blockIdx.y, p = blockIdx.z * 64 + threadIdx.x, grp = h / (g.heads / g.groups), N = g.state_dim;
-    const Seq s = seq_of(g.rows, blockIdx.x, g.state != nullptr);
-    if (s.count < 0) return;
-    const bool on = p < g.head_dim;
-    float *st = g.state ? g.state + (((size_t)s.slot * g.heads + h) * g.head_dim + p) * N : nullptr;
-    for (int n = 0; n < N; ++n) H[threadIdx.x][n] = on && st && s.pos > 0 ? st[n] : 0.0f;
-    for (int t = 0; t < s.count; ++t) {
-        const size_t row = (size_t)(s.row + t);
-        __syncthreads();
-        for (int n = threadIdx.x; n < N; n += 64) {
-            B[n] = to_f32(static_cast<const T *>(g.b)[row * g.ldb + grp * N + n]);
-            C[n] = to_f32(static_cast<const T *>(g.c)[row * g.ldc + grp * N + n]);
-        }
-        __syncthreads();
-        if (!on) continue;
-        const float delta = softplus(load_any(g.dt, row * g.lddt + h, g.dt_dtype) + (g.dt_bias ? g.dt_bias[h] : 0.0f));
-        const float decay = expf(delta * g.a[h]), x = to_f32(static_cast<const T *>(g.x)[row * g.ldx + (size_t)h * g.head_dim + p]), u = delta * x;
-        float y = 0.0f;
-        for (int n = 0; n < N; ++n) {
-            const float v = fmaf(decay, H[threadIdx.x][n], u * B[n]);
-            H[threadIdx.x][n] = v;
-            y = fmaf(v, C[n], y);
-        }
-        if (g.d) y = fmaf(g.d[h], x, y);
-        static_cast<T *>(g.y)[row * g.ldy + (size_t)h * g.head_dim + p] = from_f32<T>(y);
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, b2));
+}
+// two values -> TERMS packed bf16 pairs, each the rounding of what the ones before leave over (exact remainders)
+template <int TERMS>
+__device__ __forceinline__ void split_pair(float a, float b, unsigned (&o)[TERMS])
+{
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i) {
+        o[i] = cvt_pk_bf16(a, b);
+        a -= __uint_as_float(o[i] << 16);
+        b -= __uint_as_float(o[i] & 0xffff0000u);
     }
-    if (on && st && s.count > 0)
-        for (int n = 0; n < N; ++n) st[n] = H[threadIdx.x][n];
+}
+template <int TERMS>
+__device__ __forceinline__ void split8(const float *v, u32x4 (&o)[TERMS])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        unsigned u[TERMS];
+        split_pair<TERMS>(v[2 * i], v[2 * i + 1], u);
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k) o[k][i] = u[k];
+    }
+}
+// acc += a . b over the term pairs (i, j), i + j <= MOST, smallest first
+template <int MOST, int LA, int LB>
+__device__ __forceinline__ void product(f32x16 &acc, const u32x4 (&a)[LA], const u32x4 (&b)[LB])
+{
+#pragma unroll
+    for (int s = MOST; s >= 0; --s)
+#pragma unroll
+        for (int i = LA - 1; i >= 0; --i)
+            if (s - i >= 0 && s - i < LB)
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a[i]), __builtin_bit_cast(bf16x8, b[s - i]), acc, 0, 0, 0);
+}
+
+template <typename T> struct Terms;
+template <> struct Terms<Bf16> { static constexpr int X = 1, IN = 0, M = 2, OUT = 1; };   // terms of an input, cutoff of input x input; terms of M and S, cutoff of M x X and C x S
+template <> struct Terms<F16> { static constexpr int X = 2, IN = 1, M = 2, OUT = 1; };
+template <> struct Terms<float> { static constexpr int X = 3, IN = 2, M = 3, OUT = 2; };
+
+constexpr int SCAN_Q = 32, SCAN_WAVES = 4;
+
+struct ScanSplit {          // segments of long sequences; rows == 0: none
+    int rows, count;        // rows per segment (multiple of 64), segments per sequence (at most)
+    float *states;          // (B, count, heads, head_dim, state_dim): a segment's own end state, then its start state
+    float *decays;          // (B, count, heads): log2 of a segment's whole decay
+};
+
+template <typename T, int NT, bool STATE>
+__global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2) void k_scan(mdf_scan_args g, ScanSplit cut, int items, int unit_blocks)
+{
+    typedef Terms<T> K;
+    constexpr int TX = K::X, NS = 32 * NT + 8, JS = SCAN_Q + 8, BUF = TX == 1 ? 2 : 1;   // row strides in LDS: 8 values of padding spread the rows over the banks
+    __shared__ __align__(16) u16 Cs[STATE ? 1 : BUF][STATE ? 1 : TX][SCAN_Q][NS], Bs[STATE ? 1 : BUF][STATE ? 1 : TX][SCAN_Q][NS], Bt[BUF][TX][32 * NT][JS];
+    __shared__ __align__(16) float steps[SCAN_WAVES][2][5][SCAN_Q];   // D, c (high, low part), D 2^(c_31 - c), 2^c of two chunks
+    // Block -> (item, channels): workgroups of one item (which read the same B and C) lie on one XCD -- block b runs on XCD b mod 8 -- and close in time.
+    const int xcd = blockIdx.x & 7, place = blockIdx.x >> 3, item = (place / unit_blocks) * 8 + xcd, ub = place % unit_blocks;
+    if (item >= items) return;
+    const int b = cut.rows ? item / cut.count : item, seg = cut.rows ? item % cut.count : 0;
+    const Seq s = seq_of(g.rows, b, g.state != nullptr);
+    const int first = cut.rows ? seg * cut.rows : 0;
+    if (s.count <= first) return;                                     // skipped, without rows, or a segment the sequence does not reach
+    const int last = cut.rows && seg + 1 < cut.count ? min(first + cut.rows, s.count) : s.count;
+    if (STATE && last == s.count) return;                              // nobody starts from this segment's end
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
+    const int N = g.state_dim, P = g.head_dim, r = g.heads / g.groups, pblocks = (P + 31) / 32, per_group = (r * pblocks + SCAN_WAVES - 1) / SCAN_WAVES;
+    const int grp = ub / per_group, unit = (ub % per_group) * SCAN_WAVES + wave;
+    const bool works = unit < r * pblocks;                             // the others help with B and C
+    const int h = works ? grp * r + unit / pblocks : grp * r, p = (unit % pblocks) * 32 + l32;
+    const bool mine = works && p < P;
+    const size_t row0 = (size_t)s.row;
+    const T *xp = static_cast<const T *>(g.x) + (size_t)h * P + p;
+    const float a = g.a[h], bias = g.dt_bias ? g.dt_bias[h] : 0.0f, skip = g.d ? g.d[h] : 0.0f;
+
+    // the state, D-layout: register i of tile nt is n = 32 nt + 8 (i / 4) + 4 half + i % 4 of channel p
+    f32x16 S[NT];
+    const size_t cell = ((size_t)h * P + p) * N;
+    const size_t seg_cells = (size_t)g.heads * P * N;
+    const float *start = cut.rows ? (STATE ? nullptr : cut.states + ((size_t)b * cut.count + seg) * seg_cells) : g.state && s.pos > 0 ? g.state + (size_t)s.slot * seg_cells : nullptr;
+    float *end = STATE ? cut.states + ((size_t)b * cut.count + seg + 1) * seg_cells : g.state && last == s.count ? g.state + (size_t)s.slot * seg_cells : nullptr;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int n = 32 * nt + 8 * q + 4 * half;
+            Raw<float, 4> v = {};
+            if (start && mine) {
+                if (n + 4 <= N) v = load_raw<float, 4>(start + cell + n);
+                else
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (n + e < N) v.v[e] = start[cell + n + e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[nt][4 * q + e] = v.v[e];
+        }
+    double total = 0.0;                                                // log2 of the decay since `first` (STATE)
+
+    // what the next chunk needs, on its way from memory: rows 2 jp, 2 jp + 1 of B and C, values 8 nb .. 8 nb + 7; column p of X; the step sizes of two chunks
+    const int jp = threadIdx.x & 15, nb = threadIdx.x >> 4;
+    const bool stages = threadIdx.x < 64 * NT;
+    Raw<T, 8> rb[2], rc[2];
+    T rx[16];
+    float rdt = 0.0f;
+    auto fetch8 = [&](const void *base, int64_t ld, int t) {
+        Raw<T, 8> v = {};
+        const int left = N - 8 * nb;
+        if (t < last && left > 0) {
+            const T *q = static_cast<const T *>(base) + (row0 + t) * ld + (size_t)grp * N + 8 * nb;
+            if (left >= 8) v = load_raw<T, 8>(q);
+            else
+#pragma unroll
+                for (int e = 0; e < 7; ++e)
+                    if (e < left) v.v[e] = q[e];
+        }
+        return v;
+    };
+    auto request = [&](int t0) {
+        if (stages)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                rb[k] = fetch8(g.b, g.ldb, t0 + 2 * jp + k);
+                if (!STATE) rc[k] = fetch8(g.c, g.ldc, t0 + 2 * jp + k);
+            }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int t = t0 + 8 * (i / 4) + 4 * half + i % 4;
+            rx[i] = T{};
+            if (mine && t < last) rx[i] = xp[(row0 + t) * g.ldx];
+        }
+    };
+    auto request_dt = [&](int t0) { rdt = t0 + lane < last ? load_any(g.dt, (row0 + t0 + lane) * g.lddt + h, g.dt_dtype) : 0.0f; };
+    request(first);
+    request_dt(first);
+
+    for (int t0 = first, k = 0; t0 < last; t0 += SCAN_Q, ++k) {
+        const int buf = BUF == 2 ? k & 1 : 0;
+        // ---- step sizes and running log-decays of two chunks, lanes 0-31 and 32-63; the sum in double: differences of far apart rows keep their bits
+        if ((k & 1) == 0) {
+            const float D = t0 + lane < last ? softplus(rdt + bias) : 0.0f;
+            double c = (double)D * (double)a * 1.4426950408889634;
+#pragma unroll
+            for (int m = 1; m < 32; m <<= 1) {
+                const double o = __shfl_up(c, m, 32);
+                if (l32 >= m) c += o;
+            }
+            const double c31 = __shfl(c, 31, 32);
+            const float hi = (float)c;
+            steps[wave][half][0][l32] = D;
+            steps[wave][half][1][l32] = hi;
+            steps[wave][half][2][l32] = (float)(c - (double)hi);
+            steps[wave][half][3][l32] = D * __builtin_amdgcn_exp2f((float)(c31 - c));
+            steps[wave][half][4][l32] = __builtin_amdgcn_exp2f(hi);
+            if (STATE) total += __shfl(c, 31) + __shfl(c, 63);
+            request_dt(t0 + 2 * SCAN_Q);
+        }
+        // ---- this chunk's B and C into LDS, as terms
+        if (BUF == 1) __syncthreads();
+        if (stages) {
+            unsigned w[2][TX][4];   // B: row, term, pair of values
+#pragma unroll
+            for (int m = 0; m < (STATE ? 1 : 2); ++m)
+#pragma unroll
+                for (int row = 0; row < 2; ++row) {
+                    const Raw<T, 8> &v = m ? rc[row] : rb[row];
+                    unsigned u[TX][4];
+                    if constexpr (TX == 1) __builtin_memcpy(u, &v, 16);
+                    else
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            unsigned o[TX];
+                            split_pair<TX>(to_f32(v.v[2 * i]), to_f32(v.v[2 * i + 1]), o);
+#pragma unroll
+                            for (int x = 0; x < TX; ++x) u[x][i] = o[x];
+                        }
+#pragma unroll
+                    for (int x = 0; x < TX; ++x) {
+                        if constexpr (!STATE) {
+                            u16 *d = (m ? Cs : Bs)[buf][x][2 * jp + row] + 16 * (nb >> 1) + 4 * (nb & 1);
+                            *reinterpret_cast<u32x2 *>(d) = (u32x2){u[x][0], u[x][1]};
+                            *reinterpret_cast<u32x2 *>(d + 8) = (u32x2){u[x][2], u[x][3]};
+                        }
+                        if (!m)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) w[row][x][i] = u[x][i];
+                    }
+                }
+            const int j = 2 * jp, at = (j & ~12) | ((j & 4) << 1) | ((j & 8) >> 1);
+#pragma unroll
+            for (int x = 0; x < TX; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    *reinterpret_cast<unsigned *>(&Bt[buf][x][8 * nb + 2 * i][at]) = (w[0][x][i] & 0xffffu) | (w[1][x][i] << 16);
+                    *reinterpret_cast<unsigned *>(&Bt[buf][x][8 * nb + 2 * i + 1][at]) = (w[0][x][i] >> 16) | (w[1][x][i] & 0xffff0000u);
+                }
+        }
+        float xv[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) xv[i] = to_f32(rx[i]);
+        request(t0 + SCAN_Q);
+        __syncthreads();
+        if (!works) continue;
+        const float(&st)[5][SCAN_Q] = steps[wave][k & 1];
+
+        // ---- X as terms, for M X: a value that is not finite would reach rows in front of it (0 x NaN), so it counts as 0 here and spoils its own and the later
+        // rows of its channel by hand.  (What rounds to an infinite first term counts as one.)
+        u32x4 X[2][TX], W[2][3];
+        f32x16 Y;
+        int bad = SCAN_Q;
+        if constexpr (!STATE) {
+            float xs[16];
+#pragma unroll
+            for (int i = 15; i >= 0; --i) {
+                const bool ok = fabsf(xv[i]) < 0x1.ffp127f;
+                xs[i] = ok ? xv[i] : 0.0f;
+                if (!ok) bad = 8 * (i / 4) + 4 * half + i % 4;
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) split8<TX>(xs + 8 * kb, X[kb]);
+            // ---- C . S, row by row of the state, then its decay
+            f32x16 G = {};
+            Y = f32x16{};
+#pragma unroll
+            for (int kb = 0; kb < 2 * NT; ++kb) {
+                u32x4 cf[TX], bf[TX], sf[K::M];
+#pragma unroll
+                for (int x = 0; x < TX; ++x) {
+                    cf[x] = *reinterpret_cast<const u32x4 *>(&Cs[buf][x][l32][16 * kb + 8 * half]);
+                    bf[x] = *reinterpret_cast<const u32x4 *>(&Bs[buf][x][l32][16 * kb + 8 * half]);
+                }
+                float sv[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sv[e] = S[kb / 2][8 * (kb & 1) + e];
+                split8<K::M>(sv, sf);
+                product<K::IN>(G, bf, cf);     // (B C^T): lane = row i of C, registers = j
+                product<K::OUT>(Y, cf, sf);
+            }
+            // ---- M, and Y's rows
+            float m[16];
+            const float ci = st[1][l32], cl = st[2][l32];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int j0 = 8 * q + 4 * half;
+                const Raw<float, 4> D = load_raw<float, 4>(&st[0][j0]), ch = load_raw<float, 4>(&st[1][j0]), cw = load_raw<float, 4>(&st[2][j0]), ev = load_raw<float, 4>(&st[4][j0]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float v = G[4 * q + e] * (D.v[e] * __builtin_amdgcn_exp2f((ci - ch.v[e]) + (cl - cw.v[e])));
+                    m[4 * q + e] = l32 >= j0 + e ? v : 0.0f;
+                    Y[4 * q + e] *= ev.v[e];
+                }
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                u32x4 mf[K::M];
+                split8<K::M>(m + 8 * kb, mf);
+                product<K::OUT>(Y, mf, X[kb]);
+            }
+        }
+        // ---- the state
+        {
+            float w[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const Raw<float, 4> u = load_raw<float, 4>(&st[3][8 * q + 4 * half]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[4 * q + e] = u.v[e] * xv[4 * q + e];
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) split8<3>(w + 8 * kb, W[kb]);
+            const float decay = st[4][SCAN_Q - 1];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                S[nt] *= decay;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    u32x4 bf[TX];
+#pragma unroll
+                    for (int x = 0; x < TX; ++x) bf[x] = *reinterpret_cast<const u32x4 *>(&Bt[buf][x][32 * nt + l32][16 * kb + 8 * half]);
+                    product<2>(S[nt], bf, W[kb]);
+                }
+            }
+        }
+        if constexpr (!STATE) {
+            if (__any(bad < SCAN_Q)) {
+                bad = min(bad, __shfl_xor(bad, 32));
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (8 * (i / 4) + 4 * half + i % 4 >= bad) Y[i] = __builtin_nanf("");
+            }
+            if (mine) {
+                T *yp = static_cast<T *>(g.y) + (size_t)h * P + p;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int t = t0 + 8 * (i / 4) + 4 * half + i % 4;
+                    if (t < last) yp[(row0 + t) * g.ldy] = from_f32<T>(g.d ? fmaf(skip, xv[i], Y[i]) : Y[i]);
+                }
+            }
+        }
+    }
+    if (end && mine) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = 32 * nt + 8 * q + 4 * half;
+                Raw<float, 4> v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v.v[e] = S[nt][4 * q + e];
+                if (n + 4 <= N) store_raw(end + cell + n, v);
+                else
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (n + e < N) end[cell + n + e] = v.v[e];
+            }
+    }
+    if (STATE && works && lane == 0) cut.decays[((size_t)b * cut.count + seg) * g.heads + h] = (float)total;   // several waves of a head store the same value
+}
+
+// The states from segment to segment: a thread per state value; what a segment made from zero becomes what the next one starts from.
+__global__ __launch_bounds__(256) void k_scan_carry(mdf_scan_args g, ScanSplit cut)
+{
+    const int b = blockIdx.y;
+    const Seq s = seq_of(g.rows, b, g.state != nullptr);
+    const int cells = g.heads * g.head_dim * g.state_dim, i = blockIdx.x * 256 + threadIdx.x;
+    if (s.count <= 0 || i >= cells) return;
+    const int h = i / (g.head_dim * g.state_dim), segs = min((s.count + cut.rows - 1) / cut.rows, cut.count);
+    float v = g.state && s.pos > 0 ? g.state[(size_t)s.slot * cells + i] : 0.0f;
+    float *at = cut.states + (size_t)b * cut.count * cells + i;
+    const float *decay = cut.decays + (size_t)b * cut.count * g.heads + h;
+    at[0] = v;
+    for (int k = 1; k < segs; ++k) {
+        v = fmaf(__builtin_amdgcn_exp2f(decay[(size_t)(k - 1) * g.heads]), v, at[(size_t)k * cells]);
+        at[(size_t)k * cells] = v;
+    }
 }
 
 // ---- one token of many sequences -----------------------------------------------------------------------------------------------------------------------
@@ -248,7 +579,10 @@ __global__ __launch_bounds__(256) void k_step(mdf_step_args g, int rows)
     __shared__ float u[PER * MOST + 2 * 128];
     const int b = blockIdx.x, h = blockIdx.y, p0 = blockIdx.z * rows, r = g.heads / g.groups, grp = h / r, P = g.head_dim, N = g.state_dim, W = g.width;
     const int slot = g.slots ? g.slots[b] : b;
-    if (slot < 0 || slot >= g.n_slots) return;
+    if (slot < 0 || slot >= g.n_slots) {
+        for (int p = threadIdx.x; g.zero_skipped && p < min(rows, P - p0); p += 256) static_cast<T *>(g.y)[(size_t)b * g.ldy + (size_t)h * P + p0 + p] = from_f32<T>(0.0f);
+        return;
+    }
     const unsigned pos = g.positions ? (unsigned)max(g.positions[b], 0) : 0u;
     const int channels = g.heads * P + 2 * g.groups * N, count = min(rows, P - p0);
     const int lane = threadIdx.x % LN, sub = threadIdx.x / LN;
@@ -523,11 +857,50 @@ static void norm_by_width(const mdf_block_norm_args &a, hipStream_t st)
     const int width = a.dim / a.groups;
     if (width <= 512) norm_launch<T, R, 64, 1>(a, st);
     else if (width <= 1024) norm_launch<T, R, 64, 2>(a, st);
-    else if (width <= 2048) norm_launch<T, R, 64, 4>(a, st);
+    else if (width <= 2048) norm_launch<T, R, 256, 1>(a, st);
     else if (width <= 4096) norm_launch<T, R, 256, 2>(a, st);
-    else if (width <= 8192) norm_launch<T, R, 256, 4>(a, st);
+    else if (width <= 8192) norm_launch<T, R, 1024, 1>(a, st);
     else if (width <= 16384) norm_launch<T, R, 1024, 2>(a, st);
     else hipLaunchKernelGGL((k_block_norm_walk<T, R>), dim3((unsigned)a.rows, a.groups), dim3(256), 0, st, a);
+}
+
+// How a call's sequences are cut.  Unsplit there is a workgroup per sequence and four blocks of 32 channels.
+struct ScanPlan {
+    int unit_blocks, seg_rows, segs;
+    size_t state_floats, decay_floats;
+};
+static ScanPlan scan_plan(const mdf_scan_args &a)
+{
+    ScanPlan p = {};
+    const int pblocks = (a.head_dim + 31) / 32;
+    p.unit_blocks = a.groups * ((a.heads / a.groups * pblocks + SCAN_WAVES - 1) / SCAN_WAVES);
+    const int64_t blocks = (int64_t)a.rows.B * p.unit_blocks;
+    p.segs = 1;
+    if (blocks < 512 && a.rows.max_len > 512) {
+        const int64_t want = (768 + blocks - 1) / blocks;
+        int rows = (int)(((a.rows.max_len + want - 1) / want + 63) / 64 * 64);
+        if (rows < 256) rows = 256;
+        if (rows < a.rows.max_len) {
+            p.seg_rows = rows;
+            p.segs = (a.rows.max_len + rows - 1) / rows;
+            p.state_floats = (size_t)a.rows.B * p.segs * a.heads * a.head_dim * a.state_dim;
+            p.decay_floats = (size_t)a.rows.B * p.segs * a.heads;
+        }
+    }
+    return p;
+}
+
+template <typename T, int NT>
+static void scan_launch(const mdf_scan_args &a, const ScanPlan &p, void *workspace, hipStream_t st)
+{
+    ScanSplit cut = {p.seg_rows, p.segs, static_cast<float *>(workspace), static_cast<float *>(workspace) + p.state_floats};
+    const int items = a.rows.B * p.segs;
+    const dim3 grid((unsigned)((items + 7) / 8 * 8 * p.unit_blocks)), block(64 * SCAN_WAVES);
+    if (p.seg_rows) {
+        hipLaunchKernelGGL((k_scan<T, NT, true>), grid, block, 0, st, a, cut, items, p.unit_blocks);
+        hipLaunchKernelGGL(k_scan_carry, dim3((unsigned)((a.heads * a.head_dim * a.state_dim + 255) / 256), (unsigned)a.rows.B), dim3(256), 0, st, a, cut);
+    }
+    hipLaunchKernelGGL((k_scan<T, NT, false>), grid, block, 0, st, a, cut, items, p.unit_blocks);
 }
 
 template <typename T>
@@ -617,9 +990,8 @@ int mdf_causal_conv_dev(const mdf_conv_args *a, void *stream)
     return MDF_OK;
 }
 
-size_t mdf_scan_workspace_bytes(const mdf_scan_args *) { return 0; }
-
-int mdf_selective_scan_dev(const mdf_scan_args *a, void *, size_t, void *stream)
+// Every argument of the scan that does not take the device to check.
+static int check_scan(const mdf_scan_args *a)
 {
     MDF_REQUIRE(a, "selective_scan_dev: NULL argument");
     if (int rc = check_rows(a->rows, "selective_scan_dev", a->state != nullptr)) return rc;
@@ -627,8 +999,8 @@ int mdf_selective_scan_dev(const mdf_scan_args *a, void *, size_t, void *stream)
     MDF_REQUIRE(a->heads > 0 && a->heads <= 65535 && a->groups > 0 && a->heads % a->groups == 0, "selective_scan_dev: %d heads in %d groups", a->heads, a->groups);
     MDF_REQUIRE(a->head_dim >= 1 && a->head_dim <= 256 && a->state_dim >= 1 && a->state_dim <= 128, "selective_scan_dev: head_dim=%d (1..256), state_dim=%d (1..128)",
                 a->head_dim, a->state_dim);
-    if (a->rows.B == 0 || (a->rows.R == 0 && !a->state)) return MDF_OK;
-    MDF_REQUIRE((a->x && a->b && a->c && a->dt && a->y) || a->rows.R == 0, "selective_scan_dev: NULL argument");
+    if (a->rows.B == 0 || a->rows.R == 0) return MDF_OK;
+    MDF_REQUIRE(a->x && a->b && a->c && a->dt && a->y, "selective_scan_dev: NULL argument");
     MDF_REQUIRE(a->a, "selective_scan_dev: a is NULL");
     const int64_t R = a->rows.R, hp = (int64_t)a->heads * a->head_dim, gn = (int64_t)a->groups * a->state_dim;
     MDF_REQUIRE(a->ldx >= 0 && a->ldb >= 0 && a->ldc >= 0 && a->lddt >= 0 && (a->ldy >= hp || R <= 1), "selective_scan_dev: a row stride is negative or y's is below %lld", (long long)hp);
@@ -636,9 +1008,37 @@ int mdf_selective_scan_dev(const mdf_scan_args *a, void *, size_t, void *stream)
     MDF_REQUIRE(!overlap(a->x, a->ldx, hp, e, a->y, a->ldy, hp, e, R) && !overlap(a->b, a->ldb, gn, e, a->y, a->ldy, hp, e, R) &&
                     !overlap(a->c, a->ldc, gn, e, a->y, a->ldy, hp, e, R) && !overlap(a->dt, a->lddt, a->heads, dt_size(a->dt_dtype), a->y, a->ldy, hp, e, R),
                 "selective_scan_dev: y overlaps an input");
+    const ScanPlan p = scan_plan(*a);
+    MDF_REQUIRE(((int64_t)a->rows.B * p.segs + 7) / 8 * 8 * p.unit_blocks < (int64_t)1 << 31 && (int64_t)a->heads * a->head_dim * a->state_dim < (int64_t)1 << 31 && a->rows.B <= 65535 * (p.seg_rows ? 1 : 32768),
+                "selective_scan_dev: %d sequences of %d heads are too many for one call", a->rows.B, a->heads);
+    return MDF_OK;
+}
+
+size_t mdf_scan_workspace_bytes(const mdf_scan_args *a)
+{
+    if (!a || a->rows.B <= 0 || a->rows.R <= 0 || check_scan(a) != MDF_OK) return 0;
+    const ScanPlan p = scan_plan(*a);
+    return (p.state_floats + p.decay_floats) * sizeof(float);
+}
+
+int mdf_selective_scan_dev(const mdf_scan_args *a, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (int rc = check_scan(a)) return rc;
+    if (a->rows.B == 0 || a->rows.R == 0) return MDF_OK;
+    const ScanPlan p = scan_plan(*a);
+    const size_t need = (p.state_floats + p.decay_floats) * sizeof(float);
+    if (need > workspace_bytes || (need && !workspace))
+        return fail(MDF_ECAPACITY, "selective_scan_dev: workspace of %zu bytes is smaller than %zu", workspace ? workspace_bytes : 0, need);
     if (int rc = require_device()) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    MDF_BY_TYPE(a->dtype, T, hipLaunchKernelGGL(k_scan_simple<T>, dim3((unsigned)a->rows.B, a->heads, (a->head_dim + 63) / 64), dim3(64), 0, st, *a));
+    MDF_BY_TYPE(a->dtype, T, {
+        switch ((a->state_dim + 31) / 32) {
+        case 1: scan_launch<T, 1>(*a, p, workspace, st); break;
+        case 2: scan_launch<T, 2>(*a, p, workspace, st); break;
+        case 3: scan_launch<T, 3>(*a, p, workspace, st); break;
+        default: scan_launch<T, 4>(*a, p, workspace, st); break;
+        }
+    });
     MDF_HIP(hipGetLastError());
     return MDF_OK;
 }

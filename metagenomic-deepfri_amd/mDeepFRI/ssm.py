@@ -46,7 +46,7 @@ class _Step(ctypes.Structure):
     _fields_ = [("xbc", c_void_p), ("dt", c_void_p), ("conv_weight", c_void_p), ("conv_bias", c_void_p), ("a", c_void_p), ("d", c_void_p), ("dt_bias", c_void_p),
                 ("conv_state", c_void_p), ("state", c_void_p), ("slots", c_void_p), ("positions", c_void_p), ("y", c_void_p), ("ldx", c_int64), ("lddt", c_int64), ("ldy", c_int64),
                 ("B", c_int32), ("n_slots", c_int32), ("heads", c_int32), ("groups", c_int32), ("head_dim", c_int32), ("state_dim", c_int32), ("width", c_int32), ("dtype", c_int32),
-                ("dt_dtype", c_int32)]
+                ("dt_dtype", c_int32), ("zero_skipped", c_int32)]
 
 
 class _Norm(ctypes.Structure):
@@ -265,7 +265,7 @@ def selective_step(xbc, dt, a, *, conv_weight, conv_state, state, positions=None
         raise ValueError(f"{conv_state.shape[0]} convolution states beside {state.shape[0]} scan states")
     g.slots, g.positions = _indices(slots, "slots", device, n), _indices(positions, "positions", device, n)
     if out is None:
-        out = torch.empty((n, heads, head_dim), dtype=xbc.dtype, device=device) if slots is None else torch.zeros((n, heads, head_dim), dtype=xbc.dtype, device=device)
+        out, g.zero_skipped = torch.empty((n, heads, head_dim), dtype=xbc.dtype, device=device), 1
     elif out.dtype != xbc.dtype:
         raise ValueError(f"out is {out.dtype}, the input {xbc.dtype}")
     g.ldy = _matrix(out, "out", device, (heads, head_dim), n)

@@ -248,8 +248,11 @@ def test_step_skips_a_padded_batch():
     xbc, dt, a, kw = step_inputs(22, 6, 4, 1, 32, 64, 4, "bf16")
     kw["slots"] = torch.tensor([3, -1, 0, 9, 8, -5], dtype=torch.int32, device="cuda")
     out = torch.full((6, 4, 32), 7.0, dtype=torch.bfloat16, device="cuda")
+    before = {k: v.clone() for k, v in kw.items()}
     check_step(xbc, dt, a, kw, out=out)
     assert bool((out[[1, 3, 5]] == 7).all())
+    made = ssm().selective_step(xbc, dt, a, **before)
+    assert torch.equal(made[[0, 2, 4]], out[[0, 2, 4]]) and bool((made[[1, 3, 5]] == 0).all())
 
 
 def test_step_in_a_pool_whose_offsets_pass_32_bits():
