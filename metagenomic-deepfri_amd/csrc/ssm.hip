@@ -26,7 +26,19 @@ template <> __device__ __forceinline__ F16 from_f32<F16>(float x) { return {__bu
 // v_rcp_f32 is within one step: an IEEE division is ten instructions per value, and these run once per element of arrays that stream from memory
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
 __device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
-__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
+// max(v, 0) + log(1 + t), t = e^-|v|; log(1 + t) = 2 artanh(s) with s = t / (2 + t) <= 1/3, its series to s^15 (the rest is below 2^-26 of it)
+__device__ __forceinline__ float softplus(float v)
+{
+    const float t = __expf(-fabsf(v)), s = t * __builtin_amdgcn_rcpf(2.0f + t), q = s * s;
+    float r = fmaf(q, 2.0f / 15.0f, 2.0f / 13.0f);
+    r = fmaf(q, r, 2.0f / 11.0f);
+    r = fmaf(q, r, 2.0f / 9.0f);
+    r = fmaf(q, r, 2.0f / 7.0f);
+    r = fmaf(q, r, 2.0f / 5.0f);
+    r = fmaf(q, r, 2.0f / 3.0f);
+    r = fmaf(q, r, 2.0f);
+    return fmaf(s, r, v > 0.0f ? v : 0.0f * v);   // (0 v: a NaN stays one)
+}
 // one value of any of the three types, by code (uniform): the step sizes dt, which are read once per head and row
 __device__ __forceinline__ float load_any(const void *p, size_t i, int dt)
 {
@@ -215,7 +227,7 @@ __global__ __launch_bounds__(256, W <= 3 ? 3 : 2) void k_conv(mdf_conv_args g, i
 // place where the next product takes them as its k, and (B C^T) comes out transposed so that M's rows lie along lanes; the k order of those products is
 // therefore 0-3, 8-11 | 4-7, 12-15 per 16, and B, C are laid into LDS in that order (bits 2 and 3 of the index exchanged).
 // Operands are sums of bfloat16 terms: bfloat16 inputs are one, float16 two and float32 three (all exact).  M and S, which only feed rounded outputs, take two
-// terms (2^-17) for the 16-bit types and three for float32; what goes into the state takes three always, so the state is a float32 one for every type.
+// terms (2^-16) for the 16-bit types and three for float32; what goes into the state takes three always, so the state is a float32 one for every type.
 // Bound for bfloat16 by issue: per chunk and wave 52 matrix instructions (state_dim 128) and about twice their time of vector instructions.
 // Long sequences are cut into segments when there are too few (sequence, head) pairs to fill the GPU: a first launch makes each segment's state from zero
 // (STATE: no Y, no C), a small one carries the states from segment to segment, the last one makes Y.
@@ -230,15 +242,22 @@ __device__ __forceinline__ unsigned cvt_pk_bf16(float a, float b)
     typedef __bf16 b2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, b2));
 }
-// two values -> TERMS packed bf16 pairs, each the rounding of what the ones before leave over (exact remainders)
+// Two values -> TERMS packed bf16 pairs whose sum they are: each term takes the leading 8 bits of what the ones before leave over (cut off, not rounded:
+// one v_perm for the pair; v_cvt_pk_bf16_f32 takes twice the time), so three terms are exact.  The last of two terms is rounded: 2^-16.
 template <int TERMS>
 __device__ __forceinline__ void split_pair(float a, float b, unsigned (&o)[TERMS])
 {
 #pragma unroll
     for (int i = 0; i < TERMS; ++i) {
-        o[i] = cvt_pk_bf16(a, b);
-        a -= __uint_as_float(o[i] << 16);
-        b -= __uint_as_float(o[i] & 0xffff0000u);
+        if (TERMS == 2 && i == 1) {
+            o[i] = cvt_pk_bf16(a, b);
+            continue;
+        }
+        o[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);   // the upper halves
+        if (i + 1 < TERMS) {
+            a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+            b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+        }
     }
 }
 template <int TERMS>
@@ -264,12 +283,68 @@ __device__ __forceinline__ void product(f32x16 &acc, const u32x4 (&a)[LA], const
                 acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a[i]), __builtin_bit_cast(bf16x8, b[s - i]), acc, 0, 0, 0);
 }
 
+// A lane's 16 values of X (one channel, rows 8 (i / 4) + 4 half + i % 4): as read, and as the terms of a product operand
+template <typename T> struct Chunk {
+    float v[16];
+    __device__ __forceinline__ bool take(const T (&x)[16])   // whether one is not finite
+    {
+        float zero = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = to_f32(x[i]), zero = fmaf(v[i], 0.0f, zero);
+        return zero != 0.0f;
+    }
+    __device__ __forceinline__ bool finite(int i) const { return fabsf(v[i]) < __builtin_inff(); }
+    __device__ __forceinline__ void clear(int i) { v[i] = 0.0f; }
+    __device__ __forceinline__ float get(int i) const { return v[i]; }
+    template <int N> __device__ __forceinline__ void terms(int kb, u32x4 (&o)[N]) const { split8<N>(v + 8 * kb, o); }
+};
+template <> struct Chunk<Bf16> {   // packed pairs, which are the operand
+    u32x4 v[2];
+    __device__ __forceinline__ bool take(const Bf16 (&x)[16])
+    {
+        typedef u16 h2 __attribute__((ext_vector_type(2)));
+        h2 most = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const unsigned u = x[i].v | (unsigned)x[i + 1].v << 16;
+            v[i / 8][i % 8 / 2] = u;
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(h2, u & 0x7fff7fffu));
+        }
+        return max(most[0], most[1]) >= 0x7f80;
+    }
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float(i & 1 ? v[i / 8][i % 8 / 2] & 0xffff0000u : v[i / 8][i % 8 / 2] << 16); }
+    __device__ __forceinline__ bool finite(int i) const { return fabsf(get(i)) < __builtin_inff(); }
+    __device__ __forceinline__ void clear(int i) { v[i / 8][i % 8 / 2] &= i & 1 ? 0xffffu : 0xffff0000u; }
+    template <int N> __device__ __forceinline__ void terms(int kb, u32x4 (&o)[N]) const { o[0] = v[kb]; }
+};
+
 template <typename T> struct Terms;
 template <> struct Terms<Bf16> { static constexpr int X = 1, IN = 0, M = 2, OUT = 1; };   // terms of an input, cutoff of input x input; terms of M and S, cutoff of M x X and C x S
 template <> struct Terms<F16> { static constexpr int X = 2, IN = 1, M = 2, OUT = 1; };
 template <> struct Terms<float> { static constexpr int X = 3, IN = 2, M = 3, OUT = 2; };
 
 constexpr int SCAN_Q = 32, SCAN_WAVES = 4;
+
+// A value the compiler may not compute with ahead of here: what is derived from it in a loop (offsets, comparisons) is made where it is used, one instruction
+// each, instead of being kept in dozens of registers over the loop
+__device__ __forceinline__ unsigned fresh(unsigned v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// Raw buffer descriptors: an access whose byte offset lies at or behind the end is dropped, a load gives 0.
+constexpr unsigned OUTSIDE = 0x80000000u;   // an offset behind every descriptor made here, with room for the rows that are added to it
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void *p, int rows, unsigned stride, unsigned width)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)((rows - 1) * stride + width), 0x00020000);
+}
+__device__ __forceinline__ void buffer_load(float &v, __amdgpu_buffer_rsrc_t r, unsigned at) { v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0)); }
+__device__ __forceinline__ void buffer_load(Bf16 &v, __amdgpu_buffer_rsrc_t r, unsigned at) { v.v = __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0); }
+__device__ __forceinline__ void buffer_load(F16 &v, __amdgpu_buffer_rsrc_t r, unsigned at) { v.v = __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0); }
+__device__ __forceinline__ void buffer_store(float v, __amdgpu_buffer_rsrc_t r, unsigned at) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, at, 0, 0); }
+__device__ __forceinline__ void buffer_store(Bf16 v, __amdgpu_buffer_rsrc_t r, unsigned at) { __builtin_amdgcn_raw_buffer_store_b16(v.v, r, at, 0, 0); }
+__device__ __forceinline__ void buffer_store(F16 v, __amdgpu_buffer_rsrc_t r, unsigned at) { __builtin_amdgcn_raw_buffer_store_b16(v.v, r, at, 0, 0); }
 
 struct ScanSplit {          // segments of long sequences; rows == 0: none
     int rows, count;        // rows per segment (multiple of 64), segments per sequence (at most)
@@ -283,12 +358,13 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     typedef Terms<T> K;
     constexpr int TX = K::X, NS = 32 * NT + 8, JS = SCAN_Q + 8, BUF = TX == 1 ? 2 : 1;   // row strides in LDS: 8 values of padding spread the rows over the banks
     __shared__ __align__(16) u16 Cs[STATE ? 1 : BUF][STATE ? 1 : TX][SCAN_Q][NS], Bs[STATE ? 1 : BUF][STATE ? 1 : TX][SCAN_Q][NS], Bt[BUF][TX][32 * NT][JS];
-    __shared__ __align__(16) float steps[SCAN_WAVES][2][5][SCAN_Q];   // D, c (high, low part), D 2^(c_31 - c), 2^c of two chunks
+    __shared__ __align__(16) float steps[SCAN_WAVES][2][6][SCAN_Q];   // k = c - log2 D, c, low part of k, D 2^(c_31 - c), 2^c, low part of c, of two chunks
     // Block -> (item, channels): workgroups of one item (which read the same B and C) lie on one XCD -- block b runs on XCD b mod 8 -- and close in time.
     const int xcd = blockIdx.x & 7, place = blockIdx.x >> 3, item = (place / unit_blocks) * 8 + xcd, ub = place % unit_blocks;
     if (item >= items) return;
     const int b = cut.rows ? item / cut.count : item, seg = cut.rows ? item % cut.count : 0;
-    const Seq s = seq_of(g.rows, b, g.state != nullptr);
+    Seq s = seq_of(g.rows, b, g.state != nullptr);
+    s.row = __builtin_amdgcn_readfirstlane((int)s.row), s.count = __builtin_amdgcn_readfirstlane(s.count);   // the same in every lane: addresses by the scalar unit
     const int first = cut.rows ? seg * cut.rows : 0;
     if (s.count <= first) return;                                     // skipped, without rows, or a segment the sequence does not reach
     const int last = cut.rows && seg + 1 < cut.count ? min(first + cut.rows, s.count) : s.count;
@@ -300,65 +376,81 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     const int h = works ? grp * r + unit / pblocks : grp * r, p = (unit % pblocks) * 32 + l32;
     const bool mine = works && p < P;
     const size_t row0 = (size_t)s.row;
-    const T *xp = static_cast<const T *>(g.x) + (size_t)h * P + p;
     const float a = g.a[h], bias = g.dt_bias ? g.dt_bias[h] : 0.0f, skip = g.d ? g.d[h] : 0.0f;
 
     // the state, D-layout: register i of tile nt is n = 32 nt + 8 (i / 4) + 4 half + i % 4 of channel p
     f32x16 S[NT];
-    const size_t cell = ((size_t)h * P + p) * N;
-    const size_t seg_cells = (size_t)g.heads * P * N;
+    const size_t head = (size_t)h * P * N, seg_cells = (size_t)g.heads * P * N;
     const float *start = cut.rows ? (STATE ? nullptr : cut.states + ((size_t)b * cut.count + seg) * seg_cells) : g.state && s.pos > 0 ? g.state + (size_t)s.slot * seg_cells : nullptr;
     float *end = STATE ? cut.states + ((size_t)b * cut.count + seg + 1) * seg_cells : g.state && last == s.count ? g.state + (size_t)s.slot * seg_cells : nullptr;
+    auto cell = [&](int n) { return mine && n < N ? fresh((unsigned)(p * N) * 4u) + 4u * n : OUTSIDE; };   // inside the head's state
+    if (start && works) {
+        const auto sr = rows_at(start + head, 1, 0, (unsigned)(P * N) * 4u);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int n = 32 * nt + 8 * q + 4 * half;
-            Raw<float, 4> v = {};
-            if (start && mine) {
-                if (n + 4 <= N) v = load_raw<float, 4>(start + cell + n);
-                else
+            for (int q = 0; q < 4; ++q) {
+                const int n = 32 * nt + 8 * q + 4 * half;
+                if ((N & 3) == 0) {
+                    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(sr, cell(n), 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 3; ++e)
-                        if (n + e < N) v.v[e] = start[cell + n + e];
+                    for (int e = 0; e < 4; ++e) S[nt][4 * q + e] = __uint_as_float(v[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) S[nt][4 * q + e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sr, cell(n + e), 0, 0));
+                }
             }
+    } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) S[nt][4 * q + e] = v.v[e];
-        }
+        for (int nt = 0; nt < NT; ++nt) S[nt] = f32x16{};
+    }
     double total = 0.0;                                                // log2 of the decay since `first` (STATE)
 
-    // what the next chunk needs, on its way from memory: rows 2 jp, 2 jp + 1 of B and C, values 8 nb .. 8 nb + 7; column p of X; the step sizes of two chunks
+    // What the next chunk needs, on its way from memory: rows 2 jp, 2 jp + 1 of B and C, values 8 nb .. 8 nb + 7; column p of X; the step sizes of two chunks.
+    // All through buffer descriptors that end with the chunk's last row: rows behind it read as 0 and are not written, lanes without a channel neither.
     const int jp = threadIdx.x & 15, nb = threadIdx.x >> 4;
     const bool stages = threadIdx.x < 64 * NT;
-    Raw<T, 8> rb[2], rc[2];
-    T rx[16];
+    constexpr unsigned E = sizeof(T);
+    const unsigned xrow = (unsigned)g.ldx * E, yrow = (unsigned)g.ldy * E, brow = (unsigned)g.ldb * E, crow = (unsigned)g.ldc * E, width = (unsigned)(g.heads * P) * E;
+    const unsigned col = (unsigned)(h * P + p) * E, xlane = mine ? 4 * half * xrow + col : OUTSIDE, ylane = mine ? 4 * half * yrow + col : OUTSIDE;
+    const char *bp = static_cast<const char *>(g.b) + row0 * brow + (size_t)grp * N * E, *cp = static_cast<const char *>(g.c) + row0 * crow + (size_t)grp * N * E;
+    const bool wide = ((reinterpret_cast<uintptr_t>(bp) | reinterpret_cast<uintptr_t>(cp) | brow | crow) & 3) == 0;   // 16-byte loads want addresses of whole words
+    const int left = N - 8 * nb;
+    Raw<T, 8> rb[2] = {}, rc[2] = {};
+    T rx[16] = {};
     float rdt = 0.0f;
-    auto fetch8 = [&](const void *base, int64_t ld, int t) {
-        Raw<T, 8> v = {};
-        const int left = N - 8 * nb;
-        if (t < last && left > 0) {
-            const T *q = static_cast<const T *>(base) + (row0 + t) * ld + (size_t)grp * N + 8 * nb;
-            if (left >= 8) v = load_raw<T, 8>(q);
-            else
+    auto fetch8 = [&](Raw<T, 8> &v, __amdgpu_buffer_rsrc_t r, unsigned row) {
+        const unsigned at = fresh(left > 0 ? row + 8 * nb * E : OUTSIDE);
+        if (wide) {
+            u32x4 u[E / 2];
 #pragma unroll
-                for (int e = 0; e < 7; ++e)
-                    if (e < left) v.v[e] = q[e];
+            for (int i = 0; i < (int)E / 2; ++i) u[i] = __builtin_amdgcn_raw_buffer_load_b128(r, at + 16 * i, 0, 0);
+            __builtin_memcpy(&v, u, sizeof(v));
+            if (N & 7)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e >= left) v.v[e] = T{};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) buffer_load(v.v[e], r, e < left ? at + e * E : OUTSIDE);
         }
-        return v;
     };
     auto request = [&](int t0) {
-        if (stages)
+        if (t0 >= last) return;
+        const int rows = min(SCAN_Q, last - t0);
+        if (stages) {
+            const auto br = rows_at(bp + (size_t)t0 * brow, rows, brow, N * E), cr = rows_at(cp + (size_t)t0 * crow, rows, crow, N * E);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                rb[k] = fetch8(g.b, g.ldb, t0 + 2 * jp + k);
-                if (!STATE) rc[k] = fetch8(g.c, g.ldc, t0 + 2 * jp + k);
+                fetch8(rb[k], br, (2 * jp + k) * brow);
+                if (!STATE) fetch8(rc[k], cr, (2 * jp + k) * crow);
             }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int t = t0 + 8 * (i / 4) + 4 * half + i % 4;
-            rx[i] = T{};
-            if (mine && t < last) rx[i] = xp[(row0 + t) * g.ldx];
         }
+        if (!works) return;
+        const auto xr = rows_at(static_cast<const char *>(g.x) + (row0 + t0) * xrow, rows, xrow, width);
+        const unsigned xl = fresh(xlane);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) buffer_load(rx[i], xr, xl + (8 * (i / 4) + i % 4) * xrow);
     };
     auto request_dt = [&](int t0) { rdt = t0 + lane < last ? load_any(g.dt, (row0 + t0 + lane) * g.lddt + h, g.dt_dtype) : 0.0f; };
     request(first);
@@ -376,12 +468,17 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
                 if (l32 >= m) c += o;
             }
             const double c31 = __shfl(c, 31, 32);
-            const float hi = (float)c;
-            steps[wave][half][0][l32] = D;
+            // D_j 2^(c_i - c_j) = 2^(c_i - k_j), k = c - log2 D; D = 0 gives k = infinity and a factor of 0.  The logarithm as v_log and what it is off by.
+            const float lg = __builtin_amdgcn_logf(D);
+            const float off = D > 0.0f ? fmaf(D, __builtin_amdgcn_exp2f(-lg), -1.0f) * 1.44269504f : 0.0f;
+            const double kd = c - (double)lg - (double)off;
+            const float hi = (float)c, khi = (float)kd;
+            steps[wave][half][0][l32] = khi;
             steps[wave][half][1][l32] = hi;
-            steps[wave][half][2][l32] = (float)(c - (double)hi);
+            steps[wave][half][2][l32] = isinf(khi) ? 0.0f : (float)(kd - (double)khi);
             steps[wave][half][3][l32] = D * __builtin_amdgcn_exp2f((float)(c31 - c));
             steps[wave][half][4][l32] = __builtin_amdgcn_exp2f(hi);
+            steps[wave][half][5][l32] = (float)(c - (double)hi);
             if (STATE) total += __shfl(c, 31) + __shfl(c, 63);
             request_dt(t0 + 2 * SCAN_Q);
         }
@@ -425,29 +522,26 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
                     *reinterpret_cast<unsigned *>(&Bt[buf][x][8 * nb + 2 * i + 1][at]) = (w[0][x][i] >> 16) | (w[1][x][i] & 0xffff0000u);
                 }
         }
-        float xv[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) xv[i] = to_f32(rx[i]);
+        // ---- X.  A value that is not finite would reach rows in front of it in M X (0 x NaN): it counts as 0, spoils its own and the later rows of its channel by
+        // hand, and the channel's state.
+        Chunk<T> xc;
+        const bool odd = xc.take(rx);
         request(t0 + SCAN_Q);
         __syncthreads();
         if (!works) continue;
-        const float(&st)[5][SCAN_Q] = steps[wave][k & 1];
-
-        // ---- X as terms, for M X: a value that is not finite would reach rows in front of it (0 x NaN), so it counts as 0 here and spoils its own and the later
-        // rows of its channel by hand.  (What rounds to an infinite first term counts as one.)
+        const float(&st)[6][SCAN_Q] = steps[wave][k & 1];
+        int bad = SCAN_Q;
+        if (__any(odd)) {
+#pragma unroll
+            for (int i = 15; i >= 0; --i)
+                if (!xc.finite(i)) xc.clear(i), bad = 8 * (i / 4) + 4 * half + i % 4;
+            bad = min(bad, __shfl_xor(bad, 32));
+        }
         u32x4 X[2][TX], W[2][3];
         f32x16 Y;
-        int bad = SCAN_Q;
         if constexpr (!STATE) {
-            float xs[16];
 #pragma unroll
-            for (int i = 15; i >= 0; --i) {
-                const bool ok = fabsf(xv[i]) < 0x1.ffp127f;
-                xs[i] = ok ? xv[i] : 0.0f;
-                if (!ok) bad = 8 * (i / 4) + 4 * half + i % 4;
-            }
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) split8<TX>(xs + 8 * kb, X[kb]);
+            for (int kb = 0; kb < 2; ++kb) xc.terms(kb, X[kb]);
             // ---- C . S, row by row of the state, then its decay
             f32x16 G = {};
             Y = f32x16{};
@@ -468,15 +562,16 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             }
             // ---- M, and Y's rows
             float m[16];
-            const float ci = st[1][l32], cl = st[2][l32];
+            const int th = (int)fresh((unsigned)(l32 - 4 * half));
+            const float ci = st[1][l32], cl = st[5][l32];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int j0 = 8 * q + 4 * half;
-                const Raw<float, 4> D = load_raw<float, 4>(&st[0][j0]), ch = load_raw<float, 4>(&st[1][j0]), cw = load_raw<float, 4>(&st[2][j0]), ev = load_raw<float, 4>(&st[4][j0]);
+                const Raw<float, 4> kh = load_raw<float, 4>(&st[0][j0]), kl = load_raw<float, 4>(&st[2][j0]), ev = load_raw<float, 4>(&st[4][j0]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float v = G[4 * q + e] * (D.v[e] * __builtin_amdgcn_exp2f((ci - ch.v[e]) + (cl - cw.v[e])));
-                    m[4 * q + e] = l32 >= j0 + e ? v : 0.0f;
+                    const float v = G[4 * q + e] * __builtin_amdgcn_exp2f((ci - kh.v[e]) + (cl - kl.v[e]));
+                    m[4 * q + e] = th >= 8 * q + e ? v : 0.0f;
                     Y[4 * q + e] *= ev.v[e];
                 }
             }
@@ -494,8 +589,9 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             for (int q = 0; q < 4; ++q) {
                 const Raw<float, 4> u = load_raw<float, 4>(&st[3][8 * q + 4 * half]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[4 * q + e] = u.v[e] * xv[4 * q + e];
+                for (int e = 0; e < 4; ++e) w[4 * q + e] = u.v[e] * xc.get(4 * q + e);
             }
+            if (bad < SCAN_Q) w[0] = __builtin_nanf("");
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) split8<3>(w + 8 * kb, W[kb]);
             const float decay = st[4][SCAN_Q - 1];
@@ -512,36 +608,32 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             }
         }
         if constexpr (!STATE) {
-            if (__any(bad < SCAN_Q)) {
-                bad = min(bad, __shfl_xor(bad, 32));
+            if (__any(bad < SCAN_Q))
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (8 * (i / 4) + 4 * half + i % 4 >= bad) Y[i] = __builtin_nanf("");
-            }
-            if (mine) {
-                T *yp = static_cast<T *>(g.y) + (size_t)h * P + p;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int t = t0 + 8 * (i / 4) + 4 * half + i % 4;
-                    if (t < last) yp[(row0 + t) * g.ldy] = from_f32<T>(g.d ? fmaf(skip, xv[i], Y[i]) : Y[i]);
-                }
-            }
+            for (int i = 0; i < 16; ++i) Y[i] = g.d ? fmaf(skip, xc.get(i), Y[i]) : Y[i];
+            const auto yr = rows_at(static_cast<char *>(g.y) + (row0 + t0) * yrow, min(SCAN_Q, last - t0), yrow, width);
+            const unsigned yl = fresh(ylane);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) buffer_store(from_f32<T>(Y[i]), yr, yl + (8 * (i / 4) + i % 4) * yrow);
         }
     }
-    if (end && mine) {
+    if (end && works) {
+        const auto sr = rows_at(end + head, 1, 0, (unsigned)(P * N) * 4u);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int n = 32 * nt + 8 * q + 4 * half;
-                Raw<float, 4> v;
+                u32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v.v[e] = S[nt][4 * q + e];
-                if (n + 4 <= N) store_raw(end + cell + n, v);
+                for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(S[nt][4 * q + e]);
+                if ((N & 3) == 0) __builtin_amdgcn_raw_buffer_store_b128(v, sr, cell(n), 0, 0);
                 else
 #pragma unroll
-                    for (int e = 0; e < 3; ++e)
-                        if (n + e < N) end[cell + n + e] = v.v[e];
+                    for (int e = 0; e < 4; ++e) __builtin_amdgcn_raw_buffer_store_b32(v[e], sr, cell(n + e), 0, 0);
             }
     }
     if (STATE && works && lane == 0) cut.decays[((size_t)b * cut.count + seg) * g.heads + h] = (float)total;   // several waves of a head store the same value
@@ -1003,7 +1095,10 @@ static int check_scan(const mdf_scan_args *a)
     MDF_REQUIRE(a->x && a->b && a->c && a->dt && a->y, "selective_scan_dev: NULL argument");
     MDF_REQUIRE(a->a, "selective_scan_dev: a is NULL");
     const int64_t R = a->rows.R, hp = (int64_t)a->heads * a->head_dim, gn = (int64_t)a->groups * a->state_dim;
-    MDF_REQUIRE(a->ldx >= 0 && a->ldb >= 0 && a->ldc >= 0 && a->lddt >= 0 && (a->ldy >= hp || R <= 1), "selective_scan_dev: a row stride is negative or y's is below %lld", (long long)hp);
+    MDF_REQUIRE(R == 1 || (a->ldx >= hp && a->ldb >= gn && a->ldc >= gn && a->lddt >= a->heads && a->ldy >= hp), "selective_scan_dev: a row stride is below its row's width");
+    // a chunk of 32 rows is addressed with 32-bit byte offsets
+    MDF_REQUIRE(a->ldx < (int64_t)1 << 23 && a->ldb < (int64_t)1 << 23 && a->ldc < (int64_t)1 << 23 && a->ldy < (int64_t)1 << 23 && hp < (int64_t)1 << 23 && gn < (int64_t)1 << 23,
+                "selective_scan_dev: a row or its stride of 2^23 values or more");
     const size_t e = dt_size(a->dtype);
     MDF_REQUIRE(!overlap(a->x, a->ldx, hp, e, a->y, a->ldy, hp, e, R) && !overlap(a->b, a->ldb, gn, e, a->y, a->ldy, hp, e, R) &&
                     !overlap(a->c, a->ldc, gn, e, a->y, a->ldy, hp, e, R) && !overlap(a->dt, a->lddt, a->heads, dt_size(a->dt_dtype), a->y, a->ldy, hp, e, R),
@@ -1025,6 +1120,8 @@ int mdf_selective_scan_dev(const mdf_scan_args *a, void *workspace, size_t works
 {
     if (int rc = check_scan(a)) return rc;
     if (a->rows.B == 0 || a->rows.R == 0) return MDF_OK;
+    mdf_scan_args one = *a;
+    if (a->rows.R == 1) one.ldx = one.ldy = (int64_t)a->heads * a->head_dim, a = &one;   // the stride of a single row says nothing
     const ScanPlan p = scan_plan(*a);
     const size_t need = (p.state_floats + p.decay_floats) * sizeof(float);
     if (need > workspace_bytes || (need && !workspace))

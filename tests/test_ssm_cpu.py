@@ -75,6 +75,8 @@ def _set(a, kw):
     (scan, dict(a=None), "NULL"),
     (scan, dict(ldy=127), "stride"),
     (scan, dict(ldb=-1), "stride"),
+    (scan, dict(ldx=0), "stride"),
+    (scan, dict(ldc=1 << 23), "stride"),
     (scan, dict(y=P + 2), "overlaps"),
     (scan, dict(y=2 * P), "overlaps"),
     (scan, dict(state=7 * P, rows__n_slots=2), "states"),
