@@ -223,9 +223,11 @@ __global__ __launch_bounds__(256, W <= 3 ? 3 : 2) void k_conv(mdf_conv_args g, i
 //     S <- 2^c_31 S + B^T diag(D_j 2^(c_31 - c_j)) X
 // -- four products on the bf16 matrix instruction (32 x 32 x 16), all sums and the state in f32.  A wave owns 32 channels of a head and their whole
 // state (16 registers per 32 state values); four waves of a workgroup, channels of the same group of heads, share the chunk's B and C in LDS.
-// No operand goes through LDS on its way from one product to the next: the state comes out of its product with four consecutive n per lane in the very
-// place where the next product takes them as its k, and (B C^T) comes out transposed so that M's rows lie along lanes; the k order of those products is
-// therefore 0-3, 8-11 | 4-7, 12-15 per 16, and B, C are laid into LDS in that order (bits 2 and 3 of the index exchanged).
+// No operand goes through LDS on its way from one product to the next: a result register holds four consecutive rows per lane half in the very place where
+// the next product takes them as its k -- in the order 0-3, 8-11 | 4-7, 12-15 per 16, which the other operand's reads follow.  (B C^T) comes out transposed,
+// lane = i, and so does Y: a lane holds four consecutive channels of a row, which leave in 16-byte stores (with a swap between the halves for 16-bit types).
+// X comes in 16-byte loads through a tile in LDS; it and B^T are read from their rows by the transposing read.  (A value per lane and instruction, 16 loads and
+// 16 stores per chunk, cost 95 of 350 us.)
 // Operands are sums of bfloat16 terms: bfloat16 inputs are one, float16 two and float32 three (all exact).  M and S, which only feed rounded outputs, take two
 // terms (2^-16) for the 16-bit types and three for float32; what goes into the state takes three always, so the state is a float32 one for every type.
 // Bound for bfloat16 by issue: per chunk and wave 52 matrix instructions (state_dim 128) and about twice their time of vector instructions.
@@ -283,40 +285,73 @@ __device__ __forceinline__ void product(f32x16 &acc, const u32x4 (&a)[LA], const
                 acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a[i]), __builtin_bit_cast(bf16x8, b[s - i]), acc, 0, 0, 0);
 }
 
-// A lane's 16 values of X (one channel, rows 8 (i / 4) + 4 half + i % 4): as read, and as the terms of a product operand
-template <typename T> struct Chunk {
+// A lane's 16 values of X -- one channel, rows 8 (i / 4) + 4 half + i % 4 -- out of the wave's tile in LDS, and as the terms of a product operand.  16-bit
+// types come four rows at a time by the transposing read: 16 lanes read 4 rows x 16 columns and each gets one column's 4 rows.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x2 read_columns(const void *tile, int stride, int row, int column)   // rows row .. row + 3, 16 columns from `column` on, over 16 lanes
+{
+    const int l16 = threadIdx.x & 15;
+    const u16 *at = static_cast<const u16 *>(tile) + (row + (l16 >> 2)) * stride + column + 4 * (l16 & 3);
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)const_cast<u16 *>(at)));
+}
+template <typename T> struct Chunk {   // float
     float v[16];
-    __device__ __forceinline__ bool take(const T (&x)[16])   // whether one is not finite
+    __device__ __forceinline__ void take(const T *tile, int stride, int half, int l32)
     {
-        float zero = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = to_f32(x[i]), zero = fmaf(v[i], 0.0f, zero);
-        return zero != 0.0f;
+        for (int i = 0; i < 16; ++i) v[i] = tile[(8 * (i / 4) + 4 * half + i % 4) * stride + l32];
     }
     __device__ __forceinline__ bool finite(int i) const { return fabsf(v[i]) < __builtin_inff(); }
     __device__ __forceinline__ void clear(int i) { v[i] = 0.0f; }
     __device__ __forceinline__ float get(int i) const { return v[i]; }
     template <int N> __device__ __forceinline__ void terms(int kb, u32x4 (&o)[N]) const { split8<N>(v + 8 * kb, o); }
 };
-template <> struct Chunk<Bf16> {   // packed pairs, which are the operand
+template <typename T> struct Packed {   // pairs of 16-bit values
     u32x4 v[2];
-    __device__ __forceinline__ bool take(const Bf16 (&x)[16])
+    __device__ __forceinline__ void take(const T *tile, int stride, int half, int l32)
     {
-        typedef u16 h2 __attribute__((ext_vector_type(2)));
-        h2 most = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            const unsigned u = x[i].v | (unsigned)x[i + 1].v << 16;
-            v[i / 8][i % 8 / 2] = u;
-            most = __builtin_elementwise_max(most, __builtin_bit_cast(h2, u & 0x7fff7fffu));
+        for (int q = 0; q < 4; ++q) {
+            const u32x2 u = read_columns(tile, stride, 8 * q + 4 * half, l32 & 16);
+            v[q / 2][2 * (q & 1)] = u[0], v[q / 2][2 * (q & 1) + 1] = u[1];
         }
-        return max(most[0], most[1]) >= 0x7f80;
     }
-    __device__ __forceinline__ float get(int i) const { return __uint_as_float(i & 1 ? v[i / 8][i % 8 / 2] & 0xffff0000u : v[i / 8][i % 8 / 2] << 16); }
-    __device__ __forceinline__ bool finite(int i) const { return fabsf(get(i)) < __builtin_inff(); }
     __device__ __forceinline__ void clear(int i) { v[i / 8][i % 8 / 2] &= i & 1 ? 0xffffu : 0xffff0000u; }
+    __device__ __forceinline__ float get(int i) const { return to_f32(T{(u16)(i & 1 ? v[i / 8][i % 8 / 2] >> 16 : v[i / 8][i % 8 / 2])}); }
+    __device__ __forceinline__ bool finite(int i) const { return fabsf(get(i)) < __builtin_inff(); }
+};
+template <> struct Chunk<Bf16> : Packed<Bf16> {   // the pairs are the operand
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float(i & 1 ? v[i / 8][i % 8 / 2] & 0xffff0000u : v[i / 8][i % 8 / 2] << 16); }
     template <int N> __device__ __forceinline__ void terms(int kb, u32x4 (&o)[N]) const { o[0] = v[kb]; }
 };
+template <> struct Chunk<F16> : Packed<F16> {
+    template <int N> __device__ __forceinline__ void terms(int kb, u32x4 (&o)[N]) const
+    {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = get(8 * kb + e);
+        split8<N>(f, o);
+    }
+};
+// whether one of 8 values is an infinity or a NaN
+__device__ __forceinline__ bool any_odd(const Raw<float, 8> &r)
+{
+    int most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, __float_as_int(r.v[i]) & 0x7fffffff);
+    return most >= 0x7f800000;
+}
+template <typename T>
+__device__ __forceinline__ bool any_odd(const Raw<T, 8> &r)
+{
+    typedef u16 h2 __attribute__((ext_vector_type(2)));
+    h2 most = {0, 0};
+    unsigned u[4];
+    __builtin_memcpy(u, &r, sizeof(u));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(h2, u[i] & 0x7fff7fffu));
+    return max(most[0], most[1]) >= (std::is_same<T, Bf16>::value ? 0x7f80 : 0x7c00);
+}
 
 template <typename T> struct Terms;
 template <> struct Terms<Bf16> { static constexpr int X = 1, IN = 0, M = 2, OUT = 1; };   // terms of an input, cutoff of input x input; terms of M and S, cutoff of M x X and C x S
@@ -331,6 +366,19 @@ __device__ __forceinline__ unsigned fresh(unsigned v)
 {
     asm volatile("" : "+v"(v));
     return v;
+}
+
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp_f64(double v)   // another lane's value; 0 where there is none or the row is not in ROWS
+{
+    const long long u = __builtin_bit_cast(long long, v);
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (long long)((unsigned long long)hi << 32 | lo));
+}
+__device__ __forceinline__ double lane_f64(double v, int lane)
+{
+    const long long u = __builtin_bit_cast(long long, v);
+    return __builtin_bit_cast(double, (long long)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(u >> 32), lane) << 32 | (unsigned)__builtin_amdgcn_readlane((int)u, lane)));
 }
 
 // Raw buffer descriptors: an access whose byte offset lies at or behind the end is dropped, a load gives 0.
@@ -356,8 +404,9 @@ template <typename T, int NT, bool STATE>
 __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2) void k_scan(mdf_scan_args g, ScanSplit cut, int items, int unit_blocks)
 {
     typedef Terms<T> K;
-    constexpr int TX = K::X, NS = 32 * NT + 8, JS = SCAN_Q + 8, BUF = TX == 1 ? 2 : 1;   // row strides in LDS: 8 values of padding spread the rows over the banks
-    __shared__ __align__(16) u16 Cs[STATE ? 1 : BUF][STATE ? 1 : TX][SCAN_Q][NS], Bs[STATE ? 1 : BUF][STATE ? 1 : TX][SCAN_Q][NS], Bt[BUF][TX][32 * NT][JS];
+    constexpr int TX = K::X, NS = 32 * NT + 8, PS = sizeof(T) == 4 ? 36 : 40, BUF = TX == 1 ? 2 : 1;   // row strides in LDS: a little more than the rows, over the banks
+    __shared__ __align__(16) u16 Cs[STATE ? 1 : BUF][STATE ? 1 : TX][SCAN_Q][NS], Bs[BUF][TX][SCAN_Q][NS];
+    __shared__ __align__(16) T Xs[SCAN_WAVES][SCAN_Q][PS];
     __shared__ __align__(16) float steps[SCAN_WAVES][2][6][SCAN_Q];   // k = c - log2 D, c, low part of k, D 2^(c_31 - c), 2^c, low part of c, of two chunks
     // Block -> (item, channels): workgroups of one item (which read the same B and C) lie on one XCD -- block b runs on XCD b mod 8 -- and close in time.
     const int xcd = blockIdx.x & 7, place = blockIdx.x >> 3, item = (place / unit_blocks) * 8 + xcd, ub = place % unit_blocks;
@@ -406,27 +455,28 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     }
     double total = 0.0;                                                // log2 of the decay since `first` (STATE)
 
-    // What the next chunk needs, on its way from memory: rows 2 jp, 2 jp + 1 of B and C, values 8 nb .. 8 nb + 7; column p of X; the step sizes of two chunks.
-    // All through buffer descriptors that end with the chunk's last row: rows behind it read as 0 and are not written, lanes without a channel neither.
-    const int jp = threadIdx.x & 15, nb = threadIdx.x >> 4;
-    const bool stages = threadIdx.x < 64 * NT;
+    // What the next chunk needs, on its way from memory, 8 values each: PER times of B and C, twice of the wave's 32 columns of X; the step sizes of two chunks.
+    // All through buffer descriptors that end with the chunk's last row: rows behind it read as 0 and are not written.
+    constexpr int PER = (NT + 1) / 2;
     constexpr unsigned E = sizeof(T);
+    const int p0 = unit % pblocks * 32;
     const unsigned xrow = (unsigned)g.ldx * E, yrow = (unsigned)g.ldy * E, brow = (unsigned)g.ldb * E, crow = (unsigned)g.ldc * E, width = (unsigned)(g.heads * P) * E;
-    const unsigned col = (unsigned)(h * P + p) * E, xlane = mine ? 4 * half * xrow + col : OUTSIDE, ylane = mine ? 4 * half * yrow + col : OUTSIDE;
+    const unsigned col = (unsigned)(h * P + p0) * E;
     const char *bp = static_cast<const char *>(g.b) + row0 * brow + (size_t)grp * N * E, *cp = static_cast<const char *>(g.c) + row0 * crow + (size_t)grp * N * E;
-    const bool wide = ((reinterpret_cast<uintptr_t>(bp) | reinterpret_cast<uintptr_t>(cp) | brow | crow) & 3) == 0;   // 16-byte loads want addresses of whole words
-    const int left = N - 8 * nb;
-    Raw<T, 8> rb[2] = {}, rc[2] = {};
-    T rx[16] = {};
+    const char *xp = static_cast<const char *>(g.x) + row0 * xrow;
+    char *yp = static_cast<char *>(g.y) + row0 * yrow;
+    auto words = [](const void *q, unsigned row) { return ((reinterpret_cast<uintptr_t>(q) | row) & 3) == 0; };   // 16-byte accesses want addresses of whole words
+    const bool bwide = words(bp, brow) && words(cp, crow), xwide = words(xp + col, xrow), ywide = words(yp, yrow) && P % (sizeof(T) == 4 ? 4 : 8) == 0;
+    Raw<T, 8> rb[PER] = {}, rc[PER] = {}, rx[2] = {};
     float rdt = 0.0f;
-    auto fetch8 = [&](Raw<T, 8> &v, __amdgpu_buffer_rsrc_t r, unsigned row) {
-        const unsigned at = fresh(left > 0 ? row + 8 * nb * E : OUTSIDE);
+    auto fetch8 = [&](Raw<T, 8> &v, __amdgpu_buffer_rsrc_t r, unsigned offset, int left, bool wide, bool exact) {   // `left` values, 0 behind them where `exact`
+        const unsigned at = fresh(left > 0 ? offset : OUTSIDE);
         if (wide) {
             u32x4 u[E / 2];
 #pragma unroll
             for (int i = 0; i < (int)E / 2; ++i) u[i] = __builtin_amdgcn_raw_buffer_load_b128(r, at + 16 * i, 0, 0);
             __builtin_memcpy(&v, u, sizeof(v));
-            if (N & 7)
+            if (exact)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     if (e >= left) v.v[e] = T{};
@@ -438,19 +488,18 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     auto request = [&](int t0) {
         if (t0 >= last) return;
         const int rows = min(SCAN_Q, last - t0);
-        if (stages) {
-            const auto br = rows_at(bp + (size_t)t0 * brow, rows, brow, N * E), cr = rows_at(cp + (size_t)t0 * crow, rows, crow, N * E);
+        const auto br = rows_at(bp + (size_t)t0 * brow, rows, brow, N * E), cr = rows_at(cp + (size_t)t0 * crow, rows, crow, N * E);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                fetch8(rb[k], br, (2 * jp + k) * brow);
-                if (!STATE) fetch8(rc[k], cr, (2 * jp + k) * crow);
-            }
+        for (int k = 0; k < PER; ++k) {
+            const int i = threadIdx.x + 256 * k, row = i / (4 * NT), n = i % (4 * NT) * 8;
+            if (128 * NT % 256 && i >= 128 * NT) continue;
+            fetch8(rb[k], br, row * brow + n * E, N - n, bwide, N & 7);
+            if (!STATE) fetch8(rc[k], cr, row * crow + n * E, N - n, bwide, N & 7);
         }
         if (!works) return;
-        const auto xr = rows_at(static_cast<const char *>(g.x) + (row0 + t0) * xrow, rows, xrow, width);
-        const unsigned xl = fresh(xlane);
+        const auto xr = rows_at(xp + (size_t)t0 * xrow, rows, xrow, width);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) buffer_load(rx[i], xr, xl + (8 * (i / 4) + i % 4) * xrow);
+        for (int k = 0; k < 2; ++k) fetch8(rx[k], xr, (lane / 4 + 16 * k) * xrow + col + lane % 4 * 8 * E, P - p0 - lane % 4 * 8, xwide, false);
     };
     auto request_dt = [&](int t0) { rdt = t0 + lane < last ? load_any(g.dt, (row0 + t0 + lane) * g.lddt + h, g.dt_dtype) : 0.0f; };
     request(first);
@@ -462,12 +511,12 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
         if ((k & 1) == 0) {
             const float D = t0 + lane < last ? softplus(rdt + bias) : 0.0f;
             double c = (double)D * (double)a * 1.4426950408889634;
-#pragma unroll
-            for (int m = 1; m < 32; m <<= 1) {
-                const double o = __shfl_up(c, m, 32);
-                if (l32 >= m) c += o;
-            }
-            const double c31 = __shfl(c, 31, 32);
+            c += dpp_f64<0x111>(c);          // from the lane 1, 2, 4, 8 below in its row of 16 (0 from outside it) ...
+            c += dpp_f64<0x112>(c);
+            c += dpp_f64<0x114>(c);
+            c += dpp_f64<0x118>(c);
+            c += dpp_f64<0x142, 0xa>(c);     // ... and from lane 15 of the row below, into rows 1 and 3
+            const double c31 = half ? lane_f64(c, 63) : lane_f64(c, 31);
             // D_j 2^(c_i - c_j) = 2^(c_i - k_j), k = c - log2 D; D = 0 gives k = infinity and a factor of 0.  The logarithm as v_log and what it is off by.
             const float lg = __builtin_amdgcn_logf(D);
             const float off = D > 0.0f ? fmaf(D, __builtin_amdgcn_exp2f(-lg), -1.0f) * 1.44269504f : 0.0f;
@@ -479,107 +528,100 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             steps[wave][half][3][l32] = D * __builtin_amdgcn_exp2f((float)(c31 - c));
             steps[wave][half][4][l32] = __builtin_amdgcn_exp2f(hi);
             steps[wave][half][5][l32] = (float)(c - (double)hi);
-            if (STATE) total += __shfl(c, 31) + __shfl(c, 63);
+            if (STATE) total += lane_f64(c, 31) + lane_f64(c, 63);
             request_dt(t0 + 2 * SCAN_Q);
         }
         // ---- this chunk's B and C into LDS, as terms
         if (BUF == 1) __syncthreads();
-        if (stages) {
-            unsigned w[2][TX][4];   // B: row, term, pair of values
 #pragma unroll
-            for (int m = 0; m < (STATE ? 1 : 2); ++m)
+        for (int k = 0; k < PER; ++k) {
+            const int i = threadIdx.x + 256 * k, row = i / (4 * NT), n = i % (4 * NT) * 8;
+            if (128 * NT % 256 && i >= 128 * NT) continue;
 #pragma unroll
-                for (int row = 0; row < 2; ++row) {
-                    const Raw<T, 8> &v = m ? rc[row] : rb[row];
-                    unsigned u[TX][4];
-                    if constexpr (TX == 1) __builtin_memcpy(u, &v, 16);
-                    else
+            for (int m = 0; m < (STATE ? 1 : 2); ++m) {
+                const Raw<T, 8> &v = m ? rc[k] : rb[k];
+                u32x4 u[TX];
+                if constexpr (TX == 1) __builtin_memcpy(u, &v, 16);
+                else {
+                    float f[8];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            unsigned o[TX];
-                            split_pair<TX>(to_f32(v.v[2 * i]), to_f32(v.v[2 * i + 1]), o);
-#pragma unroll
-                            for (int x = 0; x < TX; ++x) u[x][i] = o[x];
-                        }
-#pragma unroll
-                    for (int x = 0; x < TX; ++x) {
-                        if constexpr (!STATE) {
-                            u16 *d = (m ? Cs : Bs)[buf][x][2 * jp + row] + 16 * (nb >> 1) + 4 * (nb & 1);
-                            *reinterpret_cast<u32x2 *>(d) = (u32x2){u[x][0], u[x][1]};
-                            *reinterpret_cast<u32x2 *>(d + 8) = (u32x2){u[x][2], u[x][3]};
-                        }
-                        if (!m)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) w[row][x][i] = u[x][i];
-                    }
+                    for (int e = 0; e < 8; ++e) f[e] = to_f32(v.v[e]);
+                    split8<TX>(f, u);
                 }
-            const int j = 2 * jp, at = (j & ~12) | ((j & 4) << 1) | ((j & 8) >> 1);
 #pragma unroll
-            for (int x = 0; x < TX; ++x)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    *reinterpret_cast<unsigned *>(&Bt[buf][x][8 * nb + 2 * i][at]) = (w[0][x][i] & 0xffffu) | (w[1][x][i] << 16);
-                    *reinterpret_cast<unsigned *>(&Bt[buf][x][8 * nb + 2 * i + 1][at]) = (w[0][x][i] >> 16) | (w[1][x][i] & 0xffff0000u);
+                for (int x = 0; x < TX; ++x) {
+                    u16 *to = &Bs[buf][x][row][n];
+                    if constexpr (!STATE)
+                        if (m) to = &Cs[buf][x][row][n];
+                    *reinterpret_cast<u32x4 *>(to) = u[x];
                 }
+            }
         }
+        bool odd = false;
+        if (works)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                odd |= any_odd(rx[k]);
+                __builtin_memcpy(__builtin_assume_aligned(&Xs[wave][lane / 4 + 16 * k][lane % 4 * 8], 16), &rx[k], sizeof(rx[k]));
+            }
         // ---- X.  A value that is not finite would reach rows in front of it in M X (0 x NaN): it counts as 0, spoils its own and the later rows of its channel by
         // hand, and the channel's state.
-        Chunk<T> xc;
-        const bool odd = xc.take(rx);
         request(t0 + SCAN_Q);
         __syncthreads();
         if (!works) continue;
         const float(&st)[6][SCAN_Q] = steps[wave][k & 1];
+        Chunk<T> xc;
+        xc.take(&Xs[wave][0][0], PS, half, l32);
         int bad = SCAN_Q;
         if (__any(odd)) {
+            asm volatile("; a value that is not finite");   // (keeps what follows out of the ordinary path)
 #pragma unroll
             for (int i = 15; i >= 0; --i)
                 if (!xc.finite(i)) xc.clear(i), bad = 8 * (i / 4) + 4 * half + i % 4;
             bad = min(bad, __shfl_xor(bad, 32));
         }
         u32x4 X[2][TX], W[2][3];
-        f32x16 Y;
+        f32x16 Y = {};
         if constexpr (!STATE) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) xc.terms(kb, X[kb]);
-            // ---- C . S, row by row of the state, then its decay
+            // ---- C . S and B . C
             f32x16 G = {};
-            Y = f32x16{};
 #pragma unroll
             for (int kb = 0; kb < 2 * NT; ++kb) {
                 u32x4 cf[TX], bf[TX], sf[K::M];
+                auto frag = [&](const u16 *row) {   // k = 0-3, 8-11 or 4-7, 12-15 of 16
+                    const u32x2 lo = *reinterpret_cast<const u32x2 *>(row + 16 * kb + 4 * half), hi = *reinterpret_cast<const u32x2 *>(row + 16 * kb + 8 + 4 * half);
+                    return (u32x4){lo[0], lo[1], hi[0], hi[1]};
+                };
 #pragma unroll
-                for (int x = 0; x < TX; ++x) {
-                    cf[x] = *reinterpret_cast<const u32x4 *>(&Cs[buf][x][l32][16 * kb + 8 * half]);
-                    bf[x] = *reinterpret_cast<const u32x4 *>(&Bs[buf][x][l32][16 * kb + 8 * half]);
-                }
+                for (int x = 0; x < TX; ++x) cf[x] = frag(Cs[buf][x][l32]), bf[x] = frag(Bs[buf][x][l32]);
                 float sv[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sv[e] = S[kb / 2][8 * (kb & 1) + e];
                 split8<K::M>(sv, sf);
-                product<K::IN>(G, bf, cf);     // (B C^T): lane = row i of C, registers = j
-                product<K::OUT>(Y, cf, sf);
+                product<K::IN>(G, bf, cf);     // lane = row i of C, registers = j
+                product<K::OUT>(Y, sf, cf);    // lane = row i, registers = channels
             }
-            // ---- M, and Y's rows
+            // ---- M, and what it adds
             float m[16];
             const int th = (int)fresh((unsigned)(l32 - 4 * half));
-            const float ci = st[1][l32], cl = st[5][l32];
+            const float ci = st[1][l32], cl = st[5][l32], ei = st[4][l32];
+            Y *= ei;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int j0 = 8 * q + 4 * half;
-                const Raw<float, 4> kh = load_raw<float, 4>(&st[0][j0]), kl = load_raw<float, 4>(&st[2][j0]), ev = load_raw<float, 4>(&st[4][j0]);
+                const Raw<float, 4> kh = load_raw<float, 4>(&st[0][8 * q + 4 * half]), kl = load_raw<float, 4>(&st[2][8 * q + 4 * half]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float v = G[4 * q + e] * __builtin_amdgcn_exp2f((ci - kh.v[e]) + (cl - kl.v[e]));
                     m[4 * q + e] = th >= 8 * q + e ? v : 0.0f;
-                    Y[4 * q + e] *= ev.v[e];
                 }
             }
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 u32x4 mf[K::M];
                 split8<K::M>(m + 8 * kb, mf);
-                product<K::OUT>(Y, mf, X[kb]);
+                product<K::OUT>(Y, X[kb], mf);
             }
         }
         // ---- the state
@@ -602,22 +644,57 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
                 for (int kb = 0; kb < 2; ++kb) {
                     u32x4 bf[TX];
 #pragma unroll
-                    for (int x = 0; x < TX; ++x) bf[x] = *reinterpret_cast<const u32x4 *>(&Bt[buf][x][32 * nt + l32][16 * kb + 8 * half]);
+                    for (int x = 0; x < TX; ++x) {
+                        const u32x2 lo = read_columns(&Bs[buf][x][0][0], NS, 16 * kb + 4 * half, 32 * nt + (l32 & 16)), hi = read_columns(&Bs[buf][x][0][0], NS, 16 * kb + 8 + 4 * half, 32 * nt + (l32 & 16));
+                        bf[x] = (u32x4){lo[0], lo[1], hi[0], hi[1]};
+                    }
                     product<2>(S[nt], bf, W[kb]);
                 }
             }
         }
         if constexpr (!STATE) {
-            if (__any(bad < SCAN_Q))
+            if (__any(bad < SCAN_Q)) {
+                asm volatile("; a value that is not finite");
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (8 * (i / 4) + 4 * half + i % 4 >= bad) Y[i] = __builtin_nanf("");
+                    if (l32 >= __shfl(bad, 8 * (i / 4) + 4 * half + i % 4)) Y[i] = __builtin_nanf("");
+            }
+            if (g.d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) Y[i] = g.d ? fmaf(skip, xc.get(i), Y[i]) : Y[i];
-            const auto yr = rows_at(static_cast<char *>(g.y) + (row0 + t0) * yrow, min(SCAN_Q, last - t0), yrow, width);
-            const unsigned yl = fresh(ylane);
+                for (int q = 0; q < 4; ++q) {
+                    const Raw<T, 4> x = load_raw<T, 4>(static_cast<const T *>(__builtin_assume_aligned(&Xs[wave][l32][8 * q + 4 * half], 4 * sizeof(T))));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) buffer_store(from_f32<T>(Y[i]), yr, yl + (8 * (i / 4) + i % 4) * yrow);
+                    for (int e = 0; e < 4; ++e) Y[4 * q + e] = fmaf(skip, to_f32(x.v[e]), Y[4 * q + e]);
+                }
+            // ---- a row's channels out: register i is channel p0 + 8 (i / 4) + 4 half + i % 4
+            const auto yr = rows_at(yp + (size_t)t0 * yrow, min(SCAN_Q, last - t0), yrow, width);
+            const unsigned at = fresh(l32 * yrow + col);
+            if (!ywide) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int c = 8 * (i / 4) + 4 * half + i % 4;
+                    buffer_store(from_f32<T>(Y[i]), yr, p0 + c < P ? at + c * E : OUTSIDE);
+                }
+            } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    u32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(Y[4 * q + e]);
+                    __builtin_amdgcn_raw_buffer_store_b128(v, yr, p0 + 8 * q + 4 * half < P ? at + (8 * q + 4 * half) * E : OUTSIDE, 0, 0);
+                }
+            } else {
+                unsigned v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if constexpr (std::is_same<T, Bf16>::value) v[i] = cvt_pk_bf16(Y[2 * i], Y[2 * i + 1]);
+                    else v[i] = from_f32<T>(Y[2 * i]).v | (unsigned)from_f32<T>(Y[2 * i + 1]).v << 16;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {   // 8 channels from 16 i + 8 half on
+                    const auto a0 = __builtin_amdgcn_permlane32_swap(v[4 * i], v[4 * i + 2], false, false), a1 = __builtin_amdgcn_permlane32_swap(v[4 * i + 1], v[4 * i + 3], false, false);
+                    __builtin_amdgcn_raw_buffer_store_b128((u32x4){a0[0], a1[0], a0[1], a1[1]}, yr, p0 + 16 * i + 8 * half < P ? at + (16 * i + 8 * half) * E : OUTSIDE, 0, 0);
+                }
+            }
         }
     }
     if (end && works) {
