@@ -502,37 +502,34 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
         for (int k = 0; k < 2; ++k) fetch8(rx[k], xr, (lane / 4 + 16 * k) * xrow + col + lane % 4 * 8 * E, P - p0 - lane % 4 * 8, xwide, false);
     };
     auto request_dt = [&](int t0) { rdt = t0 + lane < last ? load_any(g.dt, (row0 + t0 + lane) * g.lddt + h, g.dt_dtype) : 0.0f; };
-    request(first);
-    request_dt(first);
-
-    for (int t0 = first, k = 0; t0 < last; t0 += SCAN_Q, ++k) {
-        const int buf = BUF == 2 ? k & 1 : 0;
-        // ---- step sizes and running log-decays of two chunks, lanes 0-31 and 32-63; the sum in double: differences of far apart rows keep their bits
-        if ((k & 1) == 0) {
-            const float D = t0 + lane < last ? softplus(rdt + bias) : 0.0f;
-            double c = (double)D * (double)a * 1.4426950408889634;
-            c += dpp_f64<0x111>(c);          // from the lane 1, 2, 4, 8 below in its row of 16 (0 from outside it) ...
-            c += dpp_f64<0x112>(c);
-            c += dpp_f64<0x114>(c);
-            c += dpp_f64<0x118>(c);
-            c += dpp_f64<0x142, 0xa>(c);     // ... and from lane 15 of the row below, into rows 1 and 3
-            const double c31 = half ? lane_f64(c, 63) : lane_f64(c, 31);
-            // D_j 2^(c_i - c_j) = 2^(c_i - k_j), k = c - log2 D; D = 0 gives k = infinity and a factor of 0.  The logarithm as v_log and what it is off by.
-            const float lg = __builtin_amdgcn_logf(D);
-            const float off = D > 0.0f ? fmaf(D, __builtin_amdgcn_exp2f(-lg), -1.0f) * 1.44269504f : 0.0f;
-            const double kd = c - (double)lg - (double)off;
-            const float hi = (float)c, khi = (float)kd;
-            steps[wave][half][0][l32] = khi;
-            steps[wave][half][1][l32] = hi;
-            steps[wave][half][2][l32] = isinf(khi) ? 0.0f : (float)(kd - (double)khi);
-            steps[wave][half][3][l32] = D * __builtin_amdgcn_exp2f((float)(c31 - c));
-            steps[wave][half][4][l32] = __builtin_amdgcn_exp2f(hi);
-            steps[wave][half][5][l32] = (float)(c - (double)hi);
-            if (STATE) total += lane_f64(c, 31) + lane_f64(c, 63);
-            request_dt(t0 + 2 * SCAN_Q);
-        }
-        // ---- this chunk's B and C into LDS, as terms
-        if (BUF == 1) __syncthreads();
+    // Step sizes and running log-decays of two chunks from t0 on, lanes 0-31 and 32-63; the sum in double: differences of far apart rows keep their bits
+    auto decays = [&](int t0) {
+        const float D = t0 + lane < last ? softplus(rdt + bias) : 0.0f;
+        double c = (double)D * (double)a * 1.4426950408889634;
+        c += dpp_f64<0x111>(c);          // from the lane 1, 2, 4, 8 below in its row of 16 (0 from outside it) ...
+        c += dpp_f64<0x112>(c);
+        c += dpp_f64<0x114>(c);
+        c += dpp_f64<0x118>(c);
+        c += dpp_f64<0x142, 0xa>(c);     // ... and from lane 15 of the row below, into rows 1 and 3
+        const double c31 = half ? lane_f64(c, 63) : lane_f64(c, 31);
+        // D_j 2^(c_i - c_j) = 2^(c_i - k_j), k = c - log2 D; D = 0 gives k = infinity and a factor of 0.  The logarithm as v_log and what it is off by.
+        const float lg = __builtin_amdgcn_logf(D);
+        const float off = D > 0.0f ? fmaf(D, __builtin_amdgcn_exp2f(-lg), -1.0f) * 1.44269504f : 0.0f;
+        const double kd = c - (double)lg - (double)off;
+        const float hi = (float)c, khi = (float)kd;
+        steps[wave][half][0][l32] = khi;
+        steps[wave][half][1][l32] = hi;
+        steps[wave][half][2][l32] = isinf(khi) ? 0.0f : (float)(kd - (double)khi);
+        steps[wave][half][3][l32] = D * __builtin_amdgcn_exp2f((float)(c31 - c));
+        steps[wave][half][4][l32] = __builtin_amdgcn_exp2f(hi);
+        steps[wave][half][5][l32] = (float)(c - (double)hi);
+        if (STATE) total += lane_f64(c, 31) + lane_f64(c, 63);
+        request_dt(t0 + 2 * SCAN_Q);
+    };
+    // What has arrived into LDS: B and C as terms, X as it is
+    bool odd = false;
+    auto stage = [&](int buf) {
+        odd = false;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const int i = threadIdx.x + 256 * k, row = i / (4 * NT), n = i % (4 * NT) * 8;
@@ -557,23 +554,33 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
                 }
             }
         }
-        bool odd = false;
         if (works)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 odd |= any_odd(rx[k]);
                 __builtin_memcpy(__builtin_assume_aligned(&Xs[wave][lane / 4 + 16 * k][lane % 4 * 8], 16), &rx[k], sizeof(rx[k]));
             }
+    };
+    // Loads are waited for in the order they and the stores were issued, so a chunk is staged in front of the stores of the one before it: behind them it would
+    // wait for their way to memory too, once per chunk (346 -> 2xx us).
+    request(first);
+    request_dt(first);
+    decays(first);
+    stage(0);
+    request(first + SCAN_Q);
+    for (int t0 = first, k = 0; t0 < last; t0 += SCAN_Q, ++k) {
+        const int buf = BUF == 2 ? k & 1 : 0;
+        const bool spoilt = __any(odd);
+        __syncthreads();
+        f32x16 Y = {};
+        if (works) {
         // ---- X.  A value that is not finite would reach rows in front of it in M X (0 x NaN): it counts as 0, spoils its own and the later rows of its channel by
         // hand, and the channel's state.
-        request(t0 + SCAN_Q);
-        __syncthreads();
-        if (!works) continue;
         const float(&st)[6][SCAN_Q] = steps[wave][k & 1];
         Chunk<T> xc;
         xc.take(&Xs[wave][0][0], PS, half, l32);
         int bad = SCAN_Q;
-        if (__any(odd)) {
+        if (spoilt) {
             asm volatile("; a value that is not finite");   // (keeps what follows out of the ordinary path)
 #pragma unroll
             for (int i = 15; i >= 0; --i)
@@ -581,7 +588,6 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             bad = min(bad, __shfl_xor(bad, 32));
         }
         u32x4 X[2][TX], W[2][3];
-        f32x16 Y = {};
         if constexpr (!STATE) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) xc.terms(kb, X[kb]);
@@ -666,6 +672,16 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) Y[4 * q + e] = fmaf(skip, to_f32(x.v[e]), Y[4 * q + e]);
                 }
+        }
+        }
+        if (t0 + SCAN_Q < last) {
+            if (BUF == 1) __syncthreads();
+            stage(BUF == 2 ? ~k & 1 : 0);
+            if (k & 1) decays(t0 + SCAN_Q);
+            request(t0 + 2 * SCAN_Q);
+        }
+        if constexpr (!STATE)
+        if (works) {
             // ---- a row's channels out: register i is channel p0 + 8 (i / 4) + 4 half + i % 4
             const auto yr = rows_at(yp + (size_t)t0 * yrow, min(SCAN_Q, last - t0), yrow, width);
             const unsigned at = fresh(l32 * yrow + col);
