@@ -266,13 +266,14 @@ typedef struct {
     void *out;
     int64_t ldx, ldo;            /* row strides in elements */
     int32_t channels, width, dtype, silu;
+    int32_t zero_skipped;        /* rows of a skipped sequence: zeros (1), or left as they are (0) */
 } mdf_conv_args;
 int mdf_causal_conv_dev(const mdf_conv_args *args, void *stream);
 
 /* With D = softplus(dt[t][h] + dt_bias[h]) and g = h / (heads / groups):
  *     H[p][n] <- exp(D a[h]) H[p][n] + D x[t][h][p] b[t][g][n],     y[t][h][p] = sum_n H[p][n] c[t][g][n] + d[h] x[t][h][p]
  * over every sequence; H is f32, state (n_slots, heads, head_dim, state_dim).  x, y: (R, heads, head_dim), b, c: (R, groups, state_dim), each
- * contiguous inside a row; dt (R, heads) of any of the three types.  y must not overlap an input.  head_dim 1..256, state_dim 1..128.
+ * contiguous inside a row, row strides at least a row's width; dt (R, heads) of any of the three types.  y must not overlap an input.  head_dim 1..256, state_dim 1..128.
  * Non-finite values stay where the recurrence puts them: nothing before the token or beside the channel they enter by is touched (an
  * infinity may come out as NaN). */
 typedef struct {
@@ -283,6 +284,7 @@ typedef struct {
     void *y;
     int64_t ldx, ldb, ldc, lddt, ldy;
     int32_t heads, groups, head_dim, state_dim, dtype, dt_dtype;
+    int32_t zero_skipped;           /* as in mdf_conv_args */
 } mdf_scan_args;
 size_t mdf_scan_workspace_bytes(const mdf_scan_args *args);
 int mdf_selective_scan_dev(const mdf_scan_args *args, void *workspace, size_t workspace_bytes, void *stream);

@@ -84,7 +84,8 @@ __device__ __forceinline__ void store_f32(T *p, const float *v)
 // What a kernel knows of a sequence; count < 0: skipped (its slot is outside the pool, or it has no rows)
 struct Seq {
     int64_t row;      // first row
-    int count;        // rows
+    int count;        // rows to work on
+    int rows;         // rows
     int slot;
     int64_t pos;      // tokens before
 };
@@ -95,7 +96,7 @@ __device__ __forceinline__ Seq seq_of(const mdf_seq_rows &r, int b, bool kept)
     int64_t n = r.lengths[b];
     if (s.row < 0 || s.row > r.R) n = 0;
     n = n < 0 ? 0 : n > r.R - s.row ? r.R - s.row : n;
-    s.count = (int)n;
+    s.count = s.rows = (int)n;
     s.slot = kept && r.slots ? r.slots[b] : b;
     s.pos = kept && r.positions ? r.positions[b] : 0;
     if (s.pos < 0) s.pos = 0;
@@ -122,7 +123,7 @@ __device__ __forceinline__ int seq_before(const int32_t *row_off, int B, int64_t
 constexpr int CONV_ROWS = 8;
 
 template <typename T, int V, int W>
-__global__ __launch_bounds__(256, W <= 3 ? 3 : 2) void k_conv(mdf_conv_args g, int steps, int lanes)   // lanes = channels / V, rounded up; channels >= V
+__global__ __launch_bounds__(256, W <= 3 ? 3 : W <= 7 ? 2 : 1) void k_conv(mdf_conv_args g, int steps, int lanes)   // lanes = channels / V, rounded up; channels >= V
 {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t tile0 = id / lanes * steps;
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(256, W <= 3 ? 3 : 2) void k_conv(mdf_conv_args g, i
     const T *x = static_cast<const T *>(g.x) + c;
     T *out = static_cast<T *>(g.out) + c, *ring = static_cast<T *>(g.state) + c;
     int b = seq_before(g.rows.row_off, g.rows.B, tile0 * CONV_ROWS);
-    Seq s = {0, -1, 0, 0};
+    Seq s = {0, -1, 0, 0, 0};
     int64_t next;   // first row of the sequence behind s
     auto begin = [&]() {
         if (b >= 0) s = seq_of(g.rows, b, g.state != nullptr);
@@ -186,6 +187,10 @@ __global__ __launch_bounds__(256, W <= 3 ? 3 : 2) void k_conv(mdf_conv_args g, i
             for (int64_t r = r0; r < r1; ++r) {
                 while (r >= next) ++b, begin();
                 const int64_t t = r - s.row;
+                if (b >= 0 && s.count < 0 && t < s.rows && g.zero_skipped) {
+                    const float zero[V] = {};
+                    store_f32<T, V>(out + (size_t)r * g.ldo, zero);
+                }
                 if (b < 0 || t >= s.count) continue;
                 if (t == 0) finish(0);
                 if (t >= W - 1) mask |= 1u << (int)(r - r0);
@@ -415,6 +420,13 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     Seq s = seq_of(g.rows, b, g.state != nullptr);
     s.row = __builtin_amdgcn_readfirstlane((int)s.row), s.count = __builtin_amdgcn_readfirstlane(s.count);   // the same in every lane: addresses by the scalar unit
     const int first = cut.rows ? seg * cut.rows : 0;
+    if (!STATE && s.count < 0 && seg == 0 && g.zero_skipped) {
+        const int r = g.heads / g.groups, pblocks = (g.head_dim + 31) / 32, per_group = (r * pblocks + SCAN_WAVES - 1) / SCAN_WAVES, h0 = ub / per_group * r;
+        const int u0 = ub % per_group * SCAN_WAVES, u1 = min(u0 + SCAN_WAVES, r * pblocks) - 1;   // the workgroup's channels lie side by side
+        const int c0 = (h0 + u0 / pblocks) * g.head_dim + u0 % pblocks * 32, c1 = (h0 + u1 / pblocks) * g.head_dim + min(u1 % pblocks * 32 + 32, g.head_dim);
+        for (int t = 0; t < s.rows; ++t)
+            for (int c = c0 + threadIdx.x; c < c1; c += 64 * SCAN_WAVES) static_cast<T *>(g.y)[(size_t)(s.row + t) * g.ldy + c] = from_f32<T>(0.0f);
+    }
     if (s.count <= first) return;                                     // skipped, without rows, or a segment the sequence does not reach
     const int last = cut.rows && seg + 1 < cut.count ? min(first + cut.rows, s.count) : s.count;
     if (STATE && last == s.count) return;                              // nobody starts from this segment's end
@@ -562,7 +574,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             }
     };
     // Loads are waited for in the order they and the stores were issued, so a chunk is staged in front of the stores of the one before it: behind them it would
-    // wait for their way to memory too, once per chunk (346 -> 2xx us).
+    // wait for their way to memory too, once per chunk (346 -> 337 us).
     request(first);
     request_dt(first);
     decays(first);
@@ -1059,17 +1071,19 @@ static ScanPlan scan_plan(const mdf_scan_args &a)
     ScanPlan p = {};
     const int pblocks = (a.head_dim + 31) / 32;
     p.unit_blocks = a.groups * ((a.heads / a.groups * pblocks + SCAN_WAVES - 1) / SCAN_WAVES);
-    const int64_t blocks = (int64_t)a.rows.B * p.unit_blocks;
     p.segs = 1;
-    if (blocks < 512 && a.rows.max_len > 512) {
-        const int64_t want = (768 + blocks - 1) / blocks;
-        int rows = (int)(((a.rows.max_len + want - 1) / want + 63) / 64 * 64);
-        if (rows < 256) rows = 256;
-        if (rows < a.rows.max_len) {
+    // `even`: rows per workgroup if all were equally long, two per CU (512).  A sequence much longer than that is what a call waits for, and the calls it
+    // holds up are cut although making the states first costs half as much again: 32 768 rows of 16 heads take 162 us in 64 segments (191 in 128, 182
+    // in 32, 580 in 8); 48 mixed lengths to 1 024 of 8 heads in float32 137 us in segments of 256, 150 uncut.  Under 256 rows the carried states outweigh it.
+    const int64_t even = a.rows.R * p.unit_blocks / 512;
+    if (a.rows.max_len > 512 && (int64_t)a.rows.max_len * 2 > even * 5) {
+        const int rows = (int)std::max<int64_t>(256, (even + 63) / 64 * 64), segs = (a.rows.max_len + rows - 1) / rows;
+        const size_t cells = (size_t)a.heads * a.head_dim * a.state_dim;
+        if (segs > 1 && (size_t)a.rows.B * segs * cells <= (size_t)1 << 28) {   // (a workspace of 1 GiB)
             p.seg_rows = rows;
-            p.segs = (a.rows.max_len + rows - 1) / rows;
-            p.state_floats = (size_t)a.rows.B * p.segs * a.heads * a.head_dim * a.state_dim;
-            p.decay_floats = (size_t)a.rows.B * p.segs * a.heads;
+            p.segs = segs;
+            p.state_floats = (size_t)a.rows.B * segs * cells;
+            p.decay_floats = (size_t)a.rows.B * segs * a.heads;
         }
     }
     return p;

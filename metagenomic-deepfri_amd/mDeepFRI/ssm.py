@@ -10,8 +10,8 @@ They stand beside the recurrent and convolutional sequence models of this packag
 whose two projections are products of the caller's.  The reference has nothing of the kind; inference only: a tensor that asks for a gradient
 is refused.
 
-Tensors are torch tensors on one GPU; work is enqueued on that GPU's current stream and nothing waits for it.  Rows of no sequence are
-left as they were in an `out` that is handed in and are zero in one that is made here.  Outputs are f32, bfloat16 or float16 like their
+Tensors are torch tensors on one GPU; work is enqueued on that GPU's current stream and nothing waits for it.  Rows of no sequence and
+of a skipped one are left as they were in an `out` that is handed in and are zero in one that is made here.  Outputs are f32, bfloat16 or float16 like their
 inputs, everything in between is f32."""
 from __future__ import annotations
 
@@ -33,13 +33,13 @@ class _Rows(ctypes.Structure):
 
 class _Conv(ctypes.Structure):
     _fields_ = [("rows", _Rows), ("x", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("state", c_void_p), ("out", c_void_p), ("ldx", c_int64), ("ldo", c_int64),
-                ("channels", c_int32), ("width", c_int32), ("dtype", c_int32), ("silu", c_int32)]
+                ("channels", c_int32), ("width", c_int32), ("dtype", c_int32), ("silu", c_int32), ("zero_skipped", c_int32)]
 
 
 class _Scan(ctypes.Structure):
     _fields_ = [("rows", _Rows), ("x", c_void_p), ("b", c_void_p), ("c", c_void_p), ("dt", c_void_p), ("a", c_void_p), ("d", c_void_p), ("dt_bias", c_void_p), ("state", c_void_p),
                 ("y", c_void_p), ("ldx", c_int64), ("ldb", c_int64), ("ldc", c_int64), ("lddt", c_int64), ("ldy", c_int64), ("heads", c_int32), ("groups", c_int32),
-                ("head_dim", c_int32), ("state_dim", c_int32), ("dtype", c_int32), ("dt_dtype", c_int32)]
+                ("head_dim", c_int32), ("state_dim", c_int32), ("dtype", c_int32), ("dt_dtype", c_int32), ("zero_skipped", c_int32)]
 
 
 class _Step(ctypes.Structure):
@@ -201,6 +201,7 @@ def causal_conv(x, weight, rows: SequenceRows, *, bias=None, silu: bool = True, 
     _fill_rows(a.rows, rows, device, x.shape[0], slots, positions, state)
     if state is not None:
         a.state = _state(state, "state", device, x.dtype, (width, channels))
+    a.zero_skipped = out is None
     out = _made(out, x, rows, x.shape)
     a.ldo = _matrix(out, "out", device, (channels,), x.shape[0])
     a.x, a.out, a.channels, a.width, a.dtype, a.silu = x.data_ptr(), out.data_ptr(), channels, width, code, bool(silu)
@@ -229,6 +230,7 @@ def selective_scan(x, dt, a, b, c, rows: SequenceRows, *, d=None, dt_bias=None, 
     _fill_rows(g.rows, rows, device, total, slots, positions, state)
     if state is not None:
         g.state = _state(state, "state", device, _torch().float32, (heads, head_dim, state_dim))
+    g.zero_skipped = out is None
     out = _made(out, x, rows, x.shape)
     g.ldy = _matrix(out, "out", device, (heads, head_dim), total)
     g.x, g.dt, g.b, g.c, g.y = x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), out.data_ptr()

@@ -39,7 +39,7 @@ def ssm():
 
 
 def lens_of(kind):
-    return {"one": [1], "ones": [1, 1, 1], "tile": [32, 64, 31, 33], "ragged": [5, 0, 130, 1, 64, 63, 65, 0, 17], "long": [301]}[kind]
+    return {"one": [1], "ones": [1, 1, 1], "tile": [32, 64, 31, 33], "ragged": [5, 0, 130, 1, 64, 63, 65, 0, 17], "long": [301], "cut": [1300, 5, 0, 513, 256]}[kind]
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -89,7 +89,11 @@ def test_conv_skips_sequences_and_leaves_other_rows():
     kw["slots"] = torch.tensor([1, -1, 99, 0], dtype=torch.int32, device="cuda")
     out = torch.full_like(x, 7.0)
     got, want = check_conv(rows, x, weight, bias, kw, out=out)
-    assert got is out and bool((out[torch.from_numpy(np.isnan(want)).cuda()] == 7).all())
+    untouched = torch.from_numpy(np.isnan(want)).cuda()
+    assert got is out and bool((out[untouched] == 7).all())
+    kw["positions"].zero_()
+    made = ssm().causal_conv(x, weight, rows, bias=bias, **kw)
+    assert bool((made[untouched] == 0).all()) and not bool((made[~untouched] == 0).all())
 
 
 def test_conv_non_finite_inputs_stay_where_they_are():
@@ -136,13 +140,14 @@ def check_scan(rows, x, dt, a, b, c, kw, out=None):
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("lens, heads, groups, head_dim, state_dim, align, pad", [
     ("one", 1, 1, 1, 1, 1, 0), ("ones", 2, 1, 64, 128, 1, 0), ("ragged", 8, 1, 64, 64, 16, 0), ("ragged", 6, 3, 40, 33, 1, 0), ("tile", 4, 2, 32, 16, 1, 8), ("tile", 3, 1, 96, 128, 1, 1),
-    ("ragged", 5, 5, 17, 7, 1, 3), ("long", 2, 1, 128, 128, 1, 0), ("long", 2, 2, 256, 100, 1, 0), ("tile", 16, 1, 32, 32, 1, 0)])
+    ("ragged", 5, 5, 17, 7, 1, 3), ("long", 2, 1, 128, 128, 1, 0), ("long", 2, 2, 256, 100, 1, 0), ("tile", 16, 1, 32, 32, 1, 0),
+    ("cut", 2, 1, 32, 64, 1, 0), ("cut", 3, 3, 40, 33, 16, 1), ("cut", 4, 2, 33, 128, 1, 0)])
 def test_scan(dtype, lens, heads, groups, head_dim, state_dim, align, pad):
     check_scan(*scan_inputs(11, lens_of(lens), heads, groups, head_dim, state_dim, dtype, align, pad=pad))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("lens, heads, groups, head_dim, state_dim", [("ragged", 4, 1, 64, 128), ("ones", 6, 3, 40, 33), ("long", 3, 1, 48, 64), ("tile", 1, 1, 20, 128)])
+@pytest.mark.parametrize("lens, heads, groups, head_dim, state_dim", [("ragged", 4, 1, 64, 128), ("ones", 6, 3, 40, 33), ("long", 3, 1, 48, 64), ("tile", 1, 1, 20, 128), ("cut", 2, 1, 64, 128), ("cut", 3, 1, 17, 30)])
 def test_scan_keeps_its_state(dtype, lens, heads, groups, head_dim, state_dim):
     check_scan(*scan_inputs(12, lens_of(lens), heads, groups, head_dim, state_dim, dtype, kept=True))
 
@@ -151,6 +156,46 @@ def test_scan_without_skip_bias_and_with_other_types_of_dt():
     for dtype, dt_dtype in (("bf16", "f32"), ("f32", "bf16"), ("f16", "f16")):
         rows, x, dt, a, b, c, kw = scan_inputs(13, [70, 3], 4, 1, 32, 24, dtype, dt_dtype=dt_dtype)
         check_scan(rows, x, dt, a, b, c, {})
+
+
+def test_scan_cut_into_segments_skips_sequences_and_spoils_only_what_follows():
+    """Sequences longer than a workgroup's share: their segments run side by side and hand their states on.  A skipped one stays as it is, a NaN spoils its
+    channel from its token to the sequence's end through every later segment, and the workspace is refused when it is too small."""
+    import ctypes
+    from mDeepFRI import _hip
+    rows, x, dt, a, b, c, kw = scan_inputs(17, [900, 1500, 640], 2, 1, 32, 64, "bf16", kept=True)
+    kw["slots"] = torch.tensor([1, -1, 0], dtype=torch.int32, device="cuda")
+    out = torch.full(x.shape, 7.0, dtype=x.dtype, device="cuda")
+    got, want = check_scan(rows, x, dt, a, b, c, kw, out=out)
+    assert bool((out[900:2400] == 7).all())
+    clean = {k: v.clone() for k, v in kw.items()}
+    bad = {k: v.clone() for k, v in kw.items()}
+    clean_out = ssm().selective_scan(x, dt, a, b, c, rows, **clean)
+    spoilt = x.clone()
+    spoilt[300, 1, 9] = math.nan
+    out = ssm().selective_scan(spoilt, dt, a, b, c, rows, **bad)
+    hit = torch.zeros(x.shape, dtype=torch.bool, device="cuda")
+    hit[300:900, 1, 9] = True
+    assert torch.equal(out[~hit], clean_out[~hit]) and not torch.isfinite(out[hit]).any()
+    state_hit = torch.zeros_like(bad["state"], dtype=torch.bool)
+    state_hit[1, 1, 9] = True
+    assert torch.equal(bad["state"][~state_hit], clean["state"][~state_hit]) and not torch.isfinite(bad["state"][state_hit]).any()
+    g = ssm()._Scan()
+    g.dtype = g.dt_dtype = _hip.DT_BF16
+    g.heads, g.groups, g.head_dim, g.state_dim, g.ldx, g.ldb, g.ldc, g.lddt, g.ldy = 2, 1, 32, 64, x.stride(0), b.stride(0), c.stride(0), dt.stride(0), 64
+    g.x, g.b, g.c, g.dt, g.a, g.y = x.data_ptr(), b.data_ptr(), c.data_ptr(), dt.data_ptr(), a.data_ptr(), out.data_ptr()
+    g.rows.lengths, g.rows.row_off, g.rows.R, g.rows.B, g.rows.max_len = rows.lengths.data_ptr(), rows.row_off.data_ptr(), x.shape[0], 3, rows.max_len
+    need = _hip.lib().mdf_scan_workspace_bytes(ctypes.byref(g))
+    assert need > 0 and _hip.lib().mdf_selective_scan_dev(ctypes.byref(g), None, 0, None) == _hip.MDF_ECAPACITY
+    with pytest.raises(_hip.CapacityError, match="workspace"):
+        _hip.check(_hip.lib().mdf_selective_scan_dev(ctypes.byref(g), out.data_ptr(), need - 1, None))
+
+
+def test_scan_with_a_longest_length_that_is_too_short():
+    """max_len sizes the cut only: a longer sequence is still run to its end, states and all."""
+    rows, x, dt, a, b, c, kw = scan_inputs(18, [1700, 600], 2, 1, 32, 64, "f32", kept=True)
+    rows.max_len = 700
+    check_scan(rows, x, dt, a, b, c, kw)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -166,7 +211,12 @@ def test_scan_skips_sequences_and_leaves_other_rows():
     kw["slots"] = torch.tensor([4, -1, 6, 0], dtype=torch.int32, device="cuda")
     out = torch.full(x.shape, 7.0, dtype=x.dtype, device="cuda")
     got, want = check_scan(rows, x, dt, a, b, c, kw, out=out)
-    assert bool((out[torch.from_numpy(np.isnan(want)).cuda()] == 7).all())
+    untouched = torch.from_numpy(np.isnan(want)).cuda()
+    assert bool((out[untouched] == 7).all())
+    junk = torch.full_like(x, math.nan)
+    del junk                                             # what the allocator hands out next is full of NaN
+    made = ssm().selective_scan(x, dt, a, b, c, rows, **kw)
+    assert bool((made[untouched] == 0).all()) and torch.isfinite(made).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])

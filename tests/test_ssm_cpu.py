@@ -133,7 +133,7 @@ def test_structures_have_the_headers_layout(tmp_path):
     from conftest import ROOT
     if not shutil.which("gcc"):
         pytest.skip("needs gcc")
-    want = {"mdf_seq_rows": (ssm._Rows, "n_slots"), "mdf_conv_args": (ssm._Conv, "silu"), "mdf_scan_args": (ssm._Scan, "dt_dtype"), "mdf_step_args": (ssm._Step, "zero_skipped"),
+    want = {"mdf_seq_rows": (ssm._Rows, "n_slots"), "mdf_conv_args": (ssm._Conv, "zero_skipped"), "mdf_scan_args": (ssm._Scan, "zero_skipped"), "mdf_step_args": (ssm._Step, "zero_skipped"),
             "mdf_block_norm_args": (ssm._Norm, "eps")}
     src = '#include <stdio.h>\n#include "mdfri.h"\nint main(void){%s return 0;}' % "".join(
         'printf("%%zu %%zu\\n", sizeof(%s), offsetof(%s, %s));' % (k, k, last) for k, (_, last) in want.items())
