@@ -16,6 +16,7 @@ inputs, everything in between is f32."""
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import c_float, c_int32, c_int64, c_void_p
 
 import numpy as np
@@ -74,7 +75,7 @@ class SequenceRows:
     """Which rows belong to which sequence: `lengths` (B) and `row_off` (B+1), int32 device tensors, row_off ascending, and the longest length.
     `dense`: the sequences cover every row (an output made here then needs no zeros).  `build` makes one from host lengths and checks them."""
 
-    __slots__ = ("lengths", "row_off", "max_len", "dense")
+    __slots__ = ("lengths", "row_off", "max_len", "dense", "count", "form")
 
     def __init__(self, lengths, row_off, max_len: int, dense: bool = False):
         torch = _torch()
@@ -84,7 +85,8 @@ class SequenceRows:
             raise ValueError(f"row_off has {row_off.shape[0]} entries for {lengths.shape[0]} sequences (one more is wanted)")
         if lengths.device != row_off.device or max_len < 0:
             raise ValueError("lengths and row_off lie on different devices, or max_len is negative")
-        self.lengths, self.row_off, self.max_len, self.dense = lengths, row_off, int(max_len), dense
+        self.lengths, self.row_off, self.max_len, self.dense, self.count = lengths, row_off, int(max_len), dense, lengths.shape[0]
+        self.form = (self.count, lengths.get_device())
 
     @classmethod
     def build(cls, lengths, device="cuda", align: int = 1):
@@ -156,35 +158,76 @@ def _state(t, name: str, device, dtype, tail: tuple):
     return t.data_ptr()
 
 
-def _fill_rows(r: _Rows, rows: SequenceRows, device, total: int, slots, positions, state) -> None:
+def _check_rows(r: _Rows, rows: SequenceRows, device, total: int, slots, positions, state) -> None:
     if state is None and (slots is not None or positions is not None):
         raise ValueError("slots and positions belong to a kept state: none is given")
-    if rows.lengths.device != device:
+    if rows.lengths.device != device or rows.row_off.device != device:
         raise ValueError(f"lengths are on {rows.lengths.device}, not on {device}")
     n = rows.lengths.shape[0]
-    r.lengths, r.row_off, r.R, r.B, r.max_len = rows.lengths.data_ptr(), rows.row_off.data_ptr(), total, n, rows.max_len
-    r.slots, r.positions = _indices(slots, "slots", device, n), _indices(positions, "positions", device, n)
-    r.n_slots = 0 if state is None else state.shape[0]
+    _indices(slots, "slots", device, n), _indices(positions, "positions", device, n)
+    r.R, r.B, r.n_slots = total, n, 0 if state is None else state.shape[0]
+
+
+# What a call's checks find -- the strides, sizes and types of its argument structure -- hangs on the tensors' shapes, strides, types and devices alone, so it is
+# kept by those: the checks of a decoding step cost more than its kernel.  Addresses are filled in at every call, in front of what is kept.
+_KNOWN = ([], [], [], [])                          # per entry point: the (form, tail) of its latest kinds of calls
+
+
+def _form(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device(), t.requires_grad)
+
+
+def _flat(t):
+    """The form of a tensor that has to be contiguous."""
+    return None if t is None else (t.shape, t.is_contiguous(), t.dtype, t.get_device(), t.requires_grad)
+
+
+def _known(entry: int, form, check):
+    recent = _KNOWN[entry]
+    for known, tail in recent:                     # compared, not hashed: unequal forms part at their first entries
+        if known == form:
+            return tail
+    tail = check()
+    recent.insert(0, (form, tail))
+    del recent[16:]
+    return tail
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _grad() -> bool:
+    return _torch().is_grad_enabled()
 
 
 def _made(out, like, rows: SequenceRows, shape):
-    if out is None:
-        torch = _torch()
-        return torch.empty(shape, dtype=like.dtype, device=like.device) if rows.dense else torch.zeros(shape, dtype=like.dtype, device=like.device)
-    if out.dtype != like.dtype:
+    """(`zero_skipped` is set for an output made here, so a dense one needs no zeros)"""
+    if out is not None:
+        return out
+    return like.new_empty(shape) if rows.dense else like.new_zeros(shape)
+
+
+def _check_out(out, like) -> None:
+    if out is not None and out.dtype != like.dtype:
         raise ValueError(f"out is {out.dtype}, the input {like.dtype}")
-    return out
 
 
 def _call(fn, device, *args) -> None:
     """Runs a library entry on the device's current stream, with that device current."""
-    torch = _torch()
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        _hip.check(fn(*args, stream))
+    cuda = _torch().cuda
+    stream = cuda.current_stream(device).cuda_stream
+    if cuda.current_device() == device.index:
+        rc = fn(*args, stream)
     else:
-        with torch.cuda.device(device):
-            _hip.check(fn(*args, stream))
+        with cuda.device(device):
+            rc = fn(*args, stream)
+    if rc:
+        _hip.check(rc)
+
+
+_ROWS = "4Qqiii4x"                                 # mdf_seq_rows
+_CONV, _SCAN, _STEP, _NORM = (struct.Struct(f) for f in (_ROWS + "5Q", _ROWS + "9Q", "12Q", "10Q"))   # up to the last address of each structure
 
 
 def causal_conv(x, weight, rows: SequenceRows, *, bias=None, silu: bool = True, state=None, slots=None, positions=None, out=None):
@@ -194,18 +237,25 @@ def causal_conv(x, weight, rows: SequenceRows, *, bias=None, silu: bool = True, 
     (n_slots, width, channels) of x's type keeps the last inputs (token t at entry t mod width) from call to call: `slots` (B) says which one
     each sequence owns (default: its own number), `positions` (B) how many tokens it had before (default 0: a new sequence)."""
     device = x.device
-    code, channels, width = _dtype(x, "x"), x.shape[-1], weight.shape[0]
-    a = _Conv()
-    a.ldx = _matrix(x, "x", device, (channels,))
-    a.weight, a.bias = _vector(weight, "weight", device, (width, channels)), _vector(bias, "bias", device, (channels,))
-    _fill_rows(a.rows, rows, device, x.shape[0], slots, positions, state)
-    if state is not None:
-        a.state = _state(state, "state", device, x.dtype, (width, channels))
-    a.zero_skipped = out is None
+
+    def check():
+        a = _Conv()
+        code, channels, width = _dtype(x, "x"), x.shape[-1], weight.shape[0]
+        a.ldx = _matrix(x, "x", device, (channels,))
+        _vector(weight, "weight", device, (width, channels)), _vector(bias, "bias", device, (channels,))
+        _check_rows(a.rows, rows, device, x.shape[0], slots, positions, state)
+        if state is not None:
+            _state(state, "state", device, x.dtype, (width, channels))
+        _check_out(out, x)
+        a.ldo = channels if out is None else _matrix(out, "out", device, (channels,), x.shape[0])
+        a.channels, a.width, a.dtype, a.silu, a.zero_skipped = channels, width, code, bool(silu), out is None
+        return bytes(a)[_CONV.size:]
+
+    tail = _known(0, (_form(x), _flat(weight), _flat(bias), rows.form, _flat(state), _flat(slots), _flat(positions), _form(out), bool(silu), _grad()), check)
     out = _made(out, x, rows, x.shape)
-    a.ldo = _matrix(out, "out", device, (channels,), x.shape[0])
-    a.x, a.out, a.channels, a.width, a.dtype, a.silu = x.data_ptr(), out.data_ptr(), channels, width, code, bool(silu)
-    _call(_hip.lib().mdf_causal_conv_dev, device, ctypes.byref(a))
+    _call(_hip.lib().mdf_causal_conv_dev, device,
+          _CONV.pack(rows.lengths.data_ptr(), rows.row_off.data_ptr(), _ptr(slots), _ptr(positions), x.shape[0], rows.count, rows.max_len, 0 if state is None else state.shape[0],
+                     x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(state), out.data_ptr()) + tail)
     return out
 
 
@@ -216,29 +266,36 @@ def selective_scan(x, dt, a, b, c, rows: SequenceRows, *, d=None, dt_bias=None, 
     row strides are free; a, d, dt_bias (heads) f32.  head_dim 1..256, state_dim 1..128, heads a multiple of groups.  state (n_slots, heads,
     head_dim, state_dim) f32 is continued where positions > 0 and left behind for the next call; slots / positions as in causal_conv."""
     device = x.device
-    if x.dim() != 3 or b.dim() != 3 or dt.dim() != 2:
-        raise ValueError(f"x, b, dt have {x.dim()}, {b.dim()}, {dt.dim()} dimensions, wanted 3, 3, 2")
-    total, heads, head_dim = x.shape
-    groups, state_dim = b.shape[1:]
-    g = _Scan()
-    g.dtype, g.dt_dtype = _dtype(x, "x"), _dtype(dt, "dt")
-    if b.dtype != x.dtype or c.dtype != x.dtype:
-        raise ValueError(f"x, b, c are {x.dtype}, {b.dtype}, {c.dtype}: one type is wanted")
-    g.ldx, g.lddt = _matrix(x, "x", device, (heads, head_dim)), _matrix(dt, "dt", device, (heads,), total)
-    g.ldb, g.ldc = _matrix(b, "b", device, (groups, state_dim), total), _matrix(c, "c", device, (groups, state_dim), total)
-    g.a, g.d, g.dt_bias = _vector(a, "a", device, (heads,)), _vector(d, "d", device, (heads,)), _vector(dt_bias, "dt_bias", device, (heads,))
-    _fill_rows(g.rows, rows, device, total, slots, positions, state)
-    if state is not None:
-        g.state = _state(state, "state", device, _torch().float32, (heads, head_dim, state_dim))
-    g.zero_skipped = out is None
+
+    def check():
+        if x.dim() != 3 or b.dim() != 3 or dt.dim() != 2:
+            raise ValueError(f"x, b, dt have {x.dim()}, {b.dim()}, {dt.dim()} dimensions, wanted 3, 3, 2")
+        total, heads, head_dim = x.shape
+        groups, state_dim = b.shape[1:]
+        g = _Scan()
+        g.dtype, g.dt_dtype = _dtype(x, "x"), _dtype(dt, "dt")
+        if b.dtype != x.dtype or c.dtype != x.dtype:
+            raise ValueError(f"x, b, c are {x.dtype}, {b.dtype}, {c.dtype}: one type is wanted")
+        g.ldx, g.lddt = _matrix(x, "x", device, (heads, head_dim)), _matrix(dt, "dt", device, (heads,), total)
+        g.ldb, g.ldc = _matrix(b, "b", device, (groups, state_dim), total), _matrix(c, "c", device, (groups, state_dim), total)
+        for name, v in (("a", a), ("d", d), ("dt_bias", dt_bias)):
+            _vector(v, name, device, (heads,))
+        _check_rows(g.rows, rows, device, total, slots, positions, state)
+        if state is not None:
+            _state(state, "state", device, _torch().float32, (heads, head_dim, state_dim))
+        _check_out(out, x)
+        g.ldy = heads * head_dim if out is None else _matrix(out, "out", device, (heads, head_dim), total)
+        g.heads, g.groups, g.head_dim, g.state_dim, g.zero_skipped = heads, groups, head_dim, state_dim, out is None
+        return bytes(g)[_SCAN.size:]
+
+    tail = _known(1, (_form(x), _form(dt), _flat(a), _form(b), _form(c), rows.form, _flat(d), _flat(dt_bias), _flat(state), _flat(slots), _flat(positions), _form(out), _grad()), check)
     out = _made(out, x, rows, x.shape)
-    g.ldy = _matrix(out, "out", device, (heads, head_dim), total)
-    g.x, g.dt, g.b, g.c, g.y = x.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr(), out.data_ptr()
-    g.heads, g.groups, g.head_dim, g.state_dim = heads, groups, head_dim, state_dim
+    args = _SCAN.pack(rows.lengths.data_ptr(), rows.row_off.data_ptr(), _ptr(slots), _ptr(positions), x.shape[0], rows.count, rows.max_len, 0 if state is None else state.shape[0],
+                      x.data_ptr(), b.data_ptr(), c.data_ptr(), dt.data_ptr(), a.data_ptr(), _ptr(d), _ptr(dt_bias), _ptr(state), out.data_ptr()) + tail
     L = _hip.lib()
-    need = L.mdf_scan_workspace_bytes(ctypes.byref(g))
+    need = L.mdf_scan_workspace_bytes(args)
     work = _torch().empty(need, dtype=_torch().uint8, device=device) if need else None
-    _call(L.mdf_selective_scan_dev, device, ctypes.byref(g), work.data_ptr() if need else None, need)
+    _call(L.mdf_selective_scan_dev, device, args, _ptr(work), need)
     return out
 
 
@@ -247,33 +304,39 @@ def selective_step(xbc, dt, a, *, conv_weight, conv_state, state, positions=None
     in one launch; conv_state (n_slots, width, channels) and state (n_slots, heads, head_dim, state_dim) are updated in place.  Returns y
     (B, heads, head_dim).  The caller adds 1 to the positions of the sequences it continues."""
     device = xbc.device
-    if state.dim() != 4 or xbc.dim() != 2:
-        raise ValueError(f"state and xbc have {state.dim()}, {xbc.dim()} dimensions, wanted 4, 2")
-    torch = _torch()
-    n, channels = xbc.shape
-    heads, head_dim, state_dim = state.shape[1:]
-    groups, odd = divmod(channels - heads * head_dim, 2 * state_dim) if state_dim else (0, 1)
-    if odd or groups < 1:
-        raise ValueError(f"xbc has {channels} channels: wanted {heads} x {head_dim} and twice a multiple of {state_dim}")
-    width = conv_weight.shape[0]
-    g = _Step()
-    g.dtype, g.dt_dtype = _dtype(xbc, "xbc"), _dtype(dt, "dt")
-    g.ldx, g.lddt = _matrix(xbc, "xbc", device, (channels,)), _matrix(dt, "dt", device, (heads,), n)
-    g.conv_weight, g.conv_bias = _vector(conv_weight, "conv_weight", device, (width, channels)), _vector(conv_bias, "conv_bias", device, (channels,))
-    g.a, g.d, g.dt_bias = _vector(a, "a", device, (heads,)), _vector(d, "d", device, (heads,)), _vector(dt_bias, "dt_bias", device, (heads,))
-    g.conv_state = _state(conv_state, "conv_state", device, xbc.dtype, (width, channels))
-    g.state = _state(state, "state", device, torch.float32, (heads, head_dim, state_dim))
-    if conv_state.shape[0] != state.shape[0]:
-        raise ValueError(f"{conv_state.shape[0]} convolution states beside {state.shape[0]} scan states")
-    g.slots, g.positions = _indices(slots, "slots", device, n), _indices(positions, "positions", device, n)
+
+    def check():
+        if state.dim() != 4 or xbc.dim() != 2:
+            raise ValueError(f"state and xbc have {state.dim()}, {xbc.dim()} dimensions, wanted 4, 2")
+        n, channels = xbc.shape
+        heads, head_dim, state_dim = state.shape[1:]
+        groups, odd = divmod(channels - heads * head_dim, 2 * state_dim) if state_dim else (0, 1)
+        if odd or groups < 1:
+            raise ValueError(f"xbc has {channels} channels: wanted {heads} x {head_dim} and twice a multiple of {state_dim}")
+        width = conv_weight.shape[0]
+        g = _Step()
+        g.dtype, g.dt_dtype = _dtype(xbc, "xbc"), _dtype(dt, "dt")
+        g.ldx, g.lddt = _matrix(xbc, "xbc", device, (channels,)), _matrix(dt, "dt", device, (heads,), n)
+        _vector(conv_weight, "conv_weight", device, (width, channels)), _vector(conv_bias, "conv_bias", device, (channels,))
+        for name, v in (("a", a), ("d", d), ("dt_bias", dt_bias)):
+            _vector(v, name, device, (heads,))
+        _state(conv_state, "conv_state", device, xbc.dtype, (width, channels))
+        _state(state, "state", device, _torch().float32, (heads, head_dim, state_dim))
+        if conv_state.shape[0] != state.shape[0]:
+            raise ValueError(f"{conv_state.shape[0]} convolution states beside {state.shape[0]} scan states")
+        _indices(slots, "slots", device, n), _indices(positions, "positions", device, n)
+        _check_out(out, xbc)
+        g.ldy = heads * head_dim if out is None else _matrix(out, "out", device, (heads, head_dim), n)
+        g.B, g.n_slots, g.heads, g.groups, g.head_dim, g.state_dim, g.width, g.zero_skipped = n, state.shape[0], heads, groups, head_dim, state_dim, width, out is None
+        return bytes(g)[_STEP.size:]
+
+    tail = _known(2, (_form(xbc), _form(dt), _flat(a), _flat(conv_weight), _flat(conv_state), _flat(state), _flat(positions), _flat(slots), _flat(conv_bias), _flat(d), _flat(dt_bias),
+                      _form(out), _grad()), check)
     if out is None:
-        out, g.zero_skipped = torch.empty((n, heads, head_dim), dtype=xbc.dtype, device=device), 1
-    elif out.dtype != xbc.dtype:
-        raise ValueError(f"out is {out.dtype}, the input {xbc.dtype}")
-    g.ldy = _matrix(out, "out", device, (heads, head_dim), n)
-    g.xbc, g.dt, g.y = xbc.data_ptr(), dt.data_ptr(), out.data_ptr()
-    g.B, g.n_slots, g.heads, g.groups, g.head_dim, g.state_dim, g.width = n, state.shape[0], heads, groups, head_dim, state_dim, width
-    _call(_hip.lib().mdf_selective_step_dev, device, ctypes.byref(g))
+        out = xbc.new_empty((xbc.shape[0],) + state.shape[1:3])
+    _call(_hip.lib().mdf_selective_step_dev, device,
+          _STEP.pack(xbc.data_ptr(), dt.data_ptr(), conv_weight.data_ptr(), _ptr(conv_bias), a.data_ptr(), _ptr(d), _ptr(dt_bias), conv_state.data_ptr(), state.data_ptr(), _ptr(slots),
+                     _ptr(positions), out.data_ptr()) + tail)
     return out
 
 
@@ -288,38 +351,43 @@ def block_norm(s, *, residual=None, gate=None, gate_act: str = "silu", gate_firs
     mean with `center`; post on each of `groups` equal parts of a row.  s and gate share a type; the residual is float32 or of that type, and r has
     its type.  residual_out may be the residual itself, out may be s or the gate."""
     device = s.device
-    if s.dim() != 2:
-        raise ValueError(f"s has {s.dim()} dimensions, wanted 2")
-    if gate_act not in ACTS:
-        raise ValueError(f"gate_act {gate_act!r} is none of {sorted(ACTS)}")
-    torch = _torch()
-    rows, dim = s.shape
-    g = _Norm()
-    g.dtype, g.lds, g.s = _dtype(s, "s"), _matrix(s, "s", device, (dim,)), s.data_ptr()
-    if gate is not None:
-        if gate.dtype != s.dtype:
-            raise ValueError(f"gate is {gate.dtype}, s {s.dtype}")
-        g.gate, g.ldg = gate.data_ptr(), _matrix(gate, "gate", device, (dim,), rows)
-    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight), ("pre_bias", pre_bias), ("scale_vec", scale_vec)):
-        if t is not None:
-            setattr(g, name, _vector(t, name, device, (dim,)))
-    if residual is not None:
-        g.residual_dtype, g.residual, g.ldr = _dtype(residual, "residual"), residual.data_ptr(), _matrix(residual, "residual", device, (dim,), rows)
-        if residual_out is None:
-            residual_out = torch.empty((rows, dim), dtype=residual.dtype, device=device)
-        elif residual_out.dtype != residual.dtype:
-            raise ValueError(f"residual_out is {residual_out.dtype}, the residual {residual.dtype}")
-        g.residual_out, g.ldro = residual_out.data_ptr(), _matrix(residual_out, "residual_out", device, (dim,), rows)
-    elif residual_out is not None:
-        raise ValueError("residual_out without a residual")
-    if pre_weight is not None or residual is None:
-        if out is None:
-            out = torch.empty((rows, dim), dtype=s.dtype, device=device)
-        elif out.dtype != s.dtype:
-            raise ValueError(f"out is {out.dtype}, s {s.dtype}")
-        g.out, g.ldo = out.data_ptr(), _matrix(out, "out", device, (dim,), rows)
-    elif out is not None:
-        raise ValueError("out without a pre-norm beside a residual: there is nothing to write there")
-    g.rows, g.dim, g.groups, g.gate_act, g.gate_first, g.center, g.scale, g.eps = rows, dim, groups, ACTS[gate_act], bool(gate_first), bool(center), scale, eps
-    _call(_hip.lib().mdf_block_norm_dev, device, ctypes.byref(g))
+    has_out = pre_weight is not None or residual is None
+
+    def check():
+        if s.dim() != 2:
+            raise ValueError(f"s has {s.dim()} dimensions, wanted 2")
+        if gate_act not in ACTS:
+            raise ValueError(f"gate_act {gate_act!r} is none of {sorted(ACTS)}")
+        rows, dim = s.shape
+        g = _Norm()
+        g.dtype, g.lds = _dtype(s, "s"), _matrix(s, "s", device, (dim,))
+        if gate is not None:
+            if gate.dtype != s.dtype:
+                raise ValueError(f"gate is {gate.dtype}, s {s.dtype}")
+            g.ldg = _matrix(gate, "gate", device, (dim,), rows)
+        for name, v in (("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight), ("pre_bias", pre_bias), ("scale_vec", scale_vec)):
+            _vector(v, name, device, (dim,))
+        if residual is not None:
+            g.residual_dtype, g.ldr, g.ldro = _dtype(residual, "residual"), _matrix(residual, "residual", device, (dim,), rows), dim
+            if residual_out is not None:
+                if residual_out.dtype != residual.dtype:
+                    raise ValueError(f"residual_out is {residual_out.dtype}, the residual {residual.dtype}")
+                g.ldro = _matrix(residual_out, "residual_out", device, (dim,), rows)
+        elif residual_out is not None:
+            raise ValueError("residual_out without a residual")
+        if out is not None and not has_out:
+            raise ValueError("out without a pre-norm beside a residual: there is nothing to write there")
+        _check_out(out, s)
+        g.ldo = dim if out is None else _matrix(out, "out", device, (dim,), rows)
+        g.rows, g.dim, g.groups, g.gate_act, g.gate_first, g.center, g.scale, g.eps = rows, dim, groups, ACTS[gate_act], bool(gate_first), bool(center), scale, eps
+        return bytes(g)[_NORM.size:]
+
+    tail = _known(3, (_form(s), _form(residual), _form(gate), gate_act, bool(gate_first), _flat(post_weight), _flat(post_bias), groups, scale, _flat(scale_vec), _flat(pre_weight),
+                      _flat(pre_bias), eps, bool(center), _form(residual_out), _form(out), _grad()), check)
+    if residual_out is None and residual is not None:
+        residual_out = residual.new_empty(s.shape)
+    if out is None and has_out:
+        out = s.new_empty(s.shape)
+    _call(_hip.lib().mdf_block_norm_dev, device,
+          _NORM.pack(s.data_ptr(), _ptr(gate), _ptr(residual), _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias), _ptr(scale_vec), _ptr(residual_out), _ptr(out)) + tail)
     return residual_out, out

@@ -144,6 +144,13 @@ def test_structures_have_the_headers_layout(tmp_path):
         assert line == "%d %d" % (ctypes.sizeof(cls), getattr(cls, last).offset), k
 
 
+def test_packed_heads_match_the_structures():
+    """The addresses that every call packs end where the structures' strides begin."""
+    assert ssm._CONV.size == ssm._Conv.ldx.offset and ssm._SCAN.size == ssm._Scan.ldx.offset and ssm._STEP.size == ssm._Step.ldx.offset and ssm._NORM.size == ssm._Norm.lds.offset
+    a = ssm._Scan.from_buffer_copy(ssm._SCAN.pack(*range(1, 18)) + bytes(ctypes.sizeof(ssm._Scan) - ssm._SCAN.size))
+    assert (a.rows.lengths, a.rows.positions, a.rows.R, a.rows.B, a.rows.max_len, a.rows.n_slots, a.x, a.dt, a.state, a.y) == (1, 4, 5, 6, 7, 8, 9, 12, 16, 17)
+
+
 def test_python_layer_refuses_host_tensors_and_bad_rows():
     import torch
     rows = ssm.SequenceRows.build([3, 0, 5], device="cpu", align=16)
