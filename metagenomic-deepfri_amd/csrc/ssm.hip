@@ -405,7 +405,8 @@ struct ScanSplit {          // segments of long sequences; rows == 0: none
     float *decays;          // (B, count, heads): log2 of a segment's whole decay
 };
 
-template <typename T, int NT, bool STATE>
+// WORDS: every row of x, b and c, and every head's and group's part of it, begins on a word
+template <typename T, int NT, bool STATE, bool WORDS>
 __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2) void k_scan(mdf_scan_args g, ScanSplit cut, int items, int unit_blocks)
 {
     typedef Terms<T> K;
@@ -477,41 +478,68 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     const char *bp = static_cast<const char *>(g.b) + row0 * brow + (size_t)grp * N * E, *cp = static_cast<const char *>(g.c) + row0 * crow + (size_t)grp * N * E;
     const char *xp = static_cast<const char *>(g.x) + row0 * xrow;
     char *yp = static_cast<char *>(g.y) + row0 * yrow;
-    auto words = [](const void *q, unsigned row) { return ((reinterpret_cast<uintptr_t>(q) | row) & 3) == 0; };   // 16-byte accesses want addresses of whole words
-    const bool bwide = words(bp, brow) && words(cp, crow), xwide = words(xp + col, xrow), ywide = words(yp, yrow) && P % (sizeof(T) == 4 ? 4 : 8) == 0;
-    Raw<T, 8> rb[PER] = {}, rc[PER] = {}, rx[2] = {};
+    auto words = [](const void *q, unsigned row) { return ((reinterpret_cast<uintptr_t>(q) | row) & 3) == 0; };   // buffer accesses want addresses of whole words
+    const bool ywide = words(yp, yrow) && P % (sizeof(T) == 4 ? 4 : 8) == 0;
+    // 8 values on their way.  Where rows or bases begin inside a word (16-bit types), the five words around them; `settle`, once they are there, shifts them into
+    // place and clears what lies behind a row's end -- not here: that would wait for the load at once.
+    struct Load {
+        Raw<T, 8> v;
+        unsigned more;
+    };
+    Load rb[PER] = {}, rc[PER] = {}, rx[2] = {};
     float rdt = 0.0f;
-    auto fetch8 = [&](Raw<T, 8> &v, __amdgpu_buffer_rsrc_t r, unsigned offset, int left, bool wide, bool exact) {   // `left` values, 0 behind them where `exact`
+    auto skew = [](const void *q) { return WORDS ? 0u : (unsigned)(reinterpret_cast<uintptr_t>(q) & 3); };
+    auto whole = [&](const char *q, int rows, unsigned stride, unsigned bytes) {   // a descriptor over whole words
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(q) - skew(q), 0, (int)(((rows - 1) * stride + bytes + skew(q) + 3) & ~3u), 0x00020000);
+    };
+    auto fetch8 = [&](Load &l, __amdgpu_buffer_rsrc_t r, unsigned offset, int left) {
         const unsigned at = fresh(left > 0 ? offset : OUTSIDE);
-        if (wide) {
+        if constexpr (WORDS) {
             u32x4 u[E / 2];
 #pragma unroll
             for (int i = 0; i < (int)E / 2; ++i) u[i] = __builtin_amdgcn_raw_buffer_load_b128(r, at + 16 * i, 0, 0);
-            __builtin_memcpy(&v, u, sizeof(v));
-            if (exact)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (e >= left) v.v[e] = T{};
+            __builtin_memcpy(&l.v, u, sizeof(l.v));
         } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) buffer_load(v.v[e], r, e < left ? at + e * E : OUTSIDE);
+            const u32x4 u = __builtin_amdgcn_raw_buffer_load_b128(r, at & ~3u, 0, 0);
+            __builtin_memcpy(&l.v, &u, 16);
+            l.more = __builtin_amdgcn_raw_buffer_load_b32(r, (at & ~3u) + 16, 0, 0);
         }
+    };
+    auto settle = [&](Load &l, unsigned offset, int left, bool exact, bool there) {   // `there`: a row of the chunk (its last word may hold the next row's first value)
+        if constexpr (!WORDS) {
+            if (!there) {
+                l.v = {};
+                return;
+            }
+            unsigned u[5];
+            __builtin_memcpy(u, &l.v, 16);
+            u[4] = l.more;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = __builtin_amdgcn_alignbit(u[i + 1], u[i], (offset & 2) * 8);
+            __builtin_memcpy(&l.v, u, 16);
+        }
+        if (exact)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e >= left) l.v.v[e] = T{};
     };
     auto request = [&](int t0) {
         if (t0 >= last) return;
         const int rows = min(SCAN_Q, last - t0);
-        const auto br = rows_at(bp + (size_t)t0 * brow, rows, brow, N * E), cr = rows_at(cp + (size_t)t0 * crow, rows, crow, N * E);
+        const char *b0 = bp + (size_t)t0 * brow, *c0 = cp + (size_t)t0 * crow;
+        const auto br = whole(b0, rows, brow, N * E), cr = whole(c0, rows, crow, N * E);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const int i = threadIdx.x + 256 * k, row = i / (4 * NT), n = i % (4 * NT) * 8;
             if (128 * NT % 256 && i >= 128 * NT) continue;
-            fetch8(rb[k], br, row * brow + n * E, N - n, bwide, N & 7);
-            if (!STATE) fetch8(rc[k], cr, row * crow + n * E, N - n, bwide, N & 7);
+            fetch8(rb[k], br, skew(b0) + row * brow + n * E, N - n);
+            if (!STATE) fetch8(rc[k], cr, skew(c0) + row * crow + n * E, N - n);
         }
         if (!works) return;
-        const auto xr = rows_at(xp + (size_t)t0 * xrow, rows, xrow, width);
+        const char *x0 = xp + (size_t)t0 * xrow;
+        const auto xr = whole(x0, rows, xrow, width);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) fetch8(rx[k], xr, (lane / 4 + 16 * k) * xrow + col + lane % 4 * 8 * E, P - p0 - lane % 4 * 8, xwide, false);
+        for (int k = 0; k < 2; ++k) fetch8(rx[k], xr, skew(x0) + (lane / 4 + 16 * k) * xrow + col + lane % 4 * 8 * E, P - p0 - lane % 4 * 8);
     };
     auto request_dt = [&](int t0) { rdt = t0 + lane < last ? load_any(g.dt, (row0 + t0 + lane) * g.lddt + h, g.dt_dtype) : 0.0f; };
     // Step sizes and running log-decays of two chunks from t0 on, lanes 0-31 and 32-63; the sum in double: differences of far apart rows keep their bits
@@ -540,7 +568,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     };
     // What has arrived into LDS: B and C as terms, X as it is
     bool odd = false;
-    auto stage = [&](int buf) {
+    auto stage = [&](int buf, int t0) {
         odd = false;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
@@ -548,7 +576,9 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             if (128 * NT % 256 && i >= 128 * NT) continue;
 #pragma unroll
             for (int m = 0; m < (STATE ? 1 : 2); ++m) {
-                const Raw<T, 8> &v = m ? rc[k] : rb[k];
+                const unsigned stride = m ? crow : brow;
+                settle(m ? rc[k] : rb[k], skew((m ? cp : bp) + (size_t)t0 * stride) + row * stride + n * E, N - n, N & 7, t0 + row < last);
+                const Raw<T, 8> &v = m ? rc[k].v : rb[k].v;
                 u32x4 u[TX];
                 if constexpr (TX == 1) __builtin_memcpy(u, &v, 16);
                 else {
@@ -569,8 +599,9 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
         if (works)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                odd |= any_odd(rx[k]);
-                __builtin_memcpy(__builtin_assume_aligned(&Xs[wave][lane / 4 + 16 * k][lane % 4 * 8], 16), &rx[k], sizeof(rx[k]));
+                settle(rx[k], skew(xp + (size_t)t0 * xrow) + (lane / 4 + 16 * k) * xrow + col + lane % 4 * 8 * E, 8, false, t0 + lane / 4 + 16 * k < last);
+                odd |= any_odd(rx[k].v);
+                __builtin_memcpy(__builtin_assume_aligned(&Xs[wave][lane / 4 + 16 * k][lane % 4 * 8], 16), &rx[k].v, sizeof(rx[k].v));
             }
     };
     // Loads are waited for in the order they and the stores were issued, so a chunk is staged in front of the stores of the one before it: behind them it would
@@ -578,7 +609,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     request(first);
     request_dt(first);
     decays(first);
-    stage(0);
+    stage(0, first);
     request(first + SCAN_Q);
     for (int t0 = first, k = 0; t0 < last; t0 += SCAN_Q, ++k) {
         const int buf = BUF == 2 ? k & 1 : 0;
@@ -688,7 +719,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
         }
         if (t0 + SCAN_Q < last) {
             if (BUF == 1) __syncthreads();
-            stage(BUF == 2 ? ~k & 1 : 0);
+            stage(BUF == 2 ? ~k & 1 : 0, t0 + SCAN_Q);
             if (k & 1) decays(t0 + SCAN_Q);
             request(t0 + 2 * SCAN_Q);
         }
@@ -1089,17 +1120,37 @@ static ScanPlan scan_plan(const mdf_scan_args &a)
     return p;
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool WORDS>
 static void scan_launch(const mdf_scan_args &a, const ScanPlan &p, void *workspace, hipStream_t st)
 {
     ScanSplit cut = {p.seg_rows, p.segs, static_cast<float *>(workspace), static_cast<float *>(workspace) + p.state_floats};
     const int items = a.rows.B * p.segs;
     const dim3 grid((unsigned)((items + 7) / 8 * 8 * p.unit_blocks)), block(64 * SCAN_WAVES);
     if (p.seg_rows) {
-        hipLaunchKernelGGL((k_scan<T, NT, true>), grid, block, 0, st, a, cut, items, p.unit_blocks);
+        hipLaunchKernelGGL((k_scan<T, NT, true, WORDS>), grid, block, 0, st, a, cut, items, p.unit_blocks);
         hipLaunchKernelGGL(k_scan_carry, dim3((unsigned)((a.heads * a.head_dim * a.state_dim + 255) / 256), (unsigned)a.rows.B), dim3(256), 0, st, a, cut);
     }
-    hipLaunchKernelGGL((k_scan<T, NT, false>), grid, block, 0, st, a, cut, items, p.unit_blocks);
+    hipLaunchKernelGGL((k_scan<T, NT, false, WORDS>), grid, block, 0, st, a, cut, items, p.unit_blocks);
+}
+template <typename T, bool WORDS>
+static void scan_by_state(const mdf_scan_args &a, const ScanPlan &p, void *workspace, hipStream_t st)
+{
+    switch ((a.state_dim + 31) / 32) {
+    case 1: scan_launch<T, 1, WORDS>(a, p, workspace, st); break;
+    case 2: scan_launch<T, 2, WORDS>(a, p, workspace, st); break;
+    case 3: scan_launch<T, 3, WORDS>(a, p, workspace, st); break;
+    default: scan_launch<T, 4, WORDS>(a, p, workspace, st); break;
+    }
+}
+template <typename T>
+static void scan_by_alignment(const mdf_scan_args &a, const ScanPlan &p, void *workspace, hipStream_t st)
+{
+    if constexpr (sizeof(T) == 2) {
+        const bool words = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.b) | reinterpret_cast<uintptr_t>(a.c)) & 3) == 0 && ((a.ldx | a.ldb | a.ldc) & 1) == 0 &&
+                           (a.heads == 1 || a.head_dim % 2 == 0) && (a.groups == 1 || a.state_dim % 2 == 0);
+        if (!words) return scan_by_state<T, false>(a, p, workspace, st);
+    }
+    scan_by_state<T, true>(a, p, workspace, st);
 }
 
 template <typename T>
@@ -1228,21 +1279,14 @@ int mdf_selective_scan_dev(const mdf_scan_args *a, void *workspace, size_t works
     if (int rc = check_scan(a)) return rc;
     if (a->rows.B == 0 || a->rows.R == 0) return MDF_OK;
     mdf_scan_args one = *a;
-    if (a->rows.R == 1) one.ldx = one.ldy = (int64_t)a->heads * a->head_dim, a = &one;   // the stride of a single row says nothing
+    if (a->rows.R == 1) one.ldx = one.ldy = ((int64_t)a->heads * a->head_dim + 1) & ~1ll, one.ldb = one.ldc = ((int64_t)a->groups * a->state_dim + 1) & ~1ll, a = &one;   // the strides of a single row say nothing
     const ScanPlan p = scan_plan(*a);
     const size_t need = (p.state_floats + p.decay_floats) * sizeof(float);
     if (need > workspace_bytes || (need && !workspace))
         return fail(MDF_ECAPACITY, "selective_scan_dev: workspace of %zu bytes is smaller than %zu", workspace ? workspace_bytes : 0, need);
     if (int rc = require_device()) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    MDF_BY_TYPE(a->dtype, T, {
-        switch ((a->state_dim + 31) / 32) {
-        case 1: scan_launch<T, 1>(*a, p, workspace, st); break;
-        case 2: scan_launch<T, 2>(*a, p, workspace, st); break;
-        case 3: scan_launch<T, 3>(*a, p, workspace, st); break;
-        default: scan_launch<T, 4>(*a, p, workspace, st); break;
-        }
-    });
+    MDF_BY_TYPE(a->dtype, T, scan_by_alignment<T>(*a, p, workspace, st));
     MDF_HIP(hipGetLastError());
     return MDF_OK;
 }

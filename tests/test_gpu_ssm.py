@@ -158,6 +158,25 @@ def test_scan_without_skip_bias_and_with_other_types_of_dt():
         check_scan(rows, x, dt, a, b, c, {})
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("groups, head_dim, state_dim, pad", [(1, 32, 64, 0), (1, 33, 31, 0), (3, 17, 33, 1)])
+def test_rows_of_no_sequence_do_not_reach_results(dtype, groups, head_dim, state_dim, pad):
+    """Rows between and behind sequences full of NaN, on whole words and off them: outputs and states as with zeros there."""
+    lens = [37, 1, 0, 64, 5]
+    rows, x, dt, a, b, c, kw = scan_inputs(19, lens, 3, groups, head_dim, state_dim, dtype, align=16, kept=True, pad=pad)
+    crows, cx, weight, bias, ckw = conv_inputs(20, lens, 40 + pad, 4, dtype, align=16, kept=True, extra_cols=pad)
+    inside = torch.zeros(x.shape[0], dtype=torch.bool, device="cuda")
+    for o, n in zip(rows.row_off.tolist(), lens):
+        inside[o:o + n] = True
+    again = {k: v.clone() for k, v in kw.items()}, {k: v.clone() for k, v in ckw.items()}
+    want, cwant = ssm().selective_scan(x, dt, a, b, c, rows, **kw), ssm().causal_conv(cx, weight, crows, bias=bias, **ckw)
+    for t in (x, dt, b, c, cx):
+        t[~inside] = math.nan
+    got, cgot = ssm().selective_scan(x, dt, a, b, c, rows, **again[0]), ssm().causal_conv(cx, weight, crows, bias=bias, **again[1])
+    assert torch.equal(got, want) and torch.equal(cgot, cwant) and torch.equal(again[0]["state"], kw["state"]) and torch.equal(again[1]["state"], ckw["state"])
+    assert bool((got[~inside] == 0).all()) and bool((cgot[~inside] == 0).all())
+
+
 def test_scan_cut_into_segments_skips_sequences_and_spoils_only_what_follows():
     """Sequences longer than a workgroup's share: their segments run side by side and hand their states on.  A skipped one stays as it is, a NaN spoils its
     channel from its token to the sequence's end through every later segment, and the workspace is refused when it is too small."""
