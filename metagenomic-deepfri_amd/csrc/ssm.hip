@@ -228,8 +228,9 @@ __global__ __launch_bounds__(256, W <= 3 ? 3 : W <= 7 ? 2 : 1) void k_conv(mdf_c
 //     S <- 2^c_31 S + B^T diag(D_j 2^(c_31 - c_j)) X
 // -- four products on the bf16 matrix instruction (32 x 32 x 16), all sums and the state in f32.  A wave owns 32 channels of a head and their whole
 // state (16 registers per 32 state values); four waves of a workgroup, channels of the same group of heads, share the chunk's B and C in LDS.
-// No operand goes through LDS on its way from one product to the next: a result register holds four consecutive rows per lane half in the very place where
-// the next product takes them as its k -- in the order 0-3, 8-11 | 4-7, 12-15 per 16, which the other operand's reads follow.  (B C^T) comes out transposed,
+// No operand goes through LDS on its way from one product to the next: result registers hold, per lane half, four consecutive rows in the very place where
+// the next product takes them as its k.  For M that order is 0-3, 8-11 | 4-7, 12-15 per 16, and X is read in it; the state's rows are put in such an order by
+// the reads of B^T that its registers are k in their natural order and C is read as it lies.  (B C^T) comes out transposed,
 // lane = i, and so does Y: a lane holds four consecutive channels of a row, which leave in 16-byte stores (with a swap between the halves for 16-bit types).
 // X comes in 16-byte loads through a tile in LDS; it and B^T are read from their rows by the transposing read.  (A value per lane and instruction, 16 loads and
 // 16 stores per chunk, cost 95 of 350 us.)
@@ -293,10 +294,11 @@ __device__ __forceinline__ void product(f32x16 &acc, const u32x4 (&a)[LA], const
 // A lane's 16 values of X -- one channel, rows 8 (i / 4) + 4 half + i % 4 -- out of the wave's tile in LDS, and as the terms of a product operand.  16-bit
 // types come four rows at a time by the transposing read: 16 lanes read 4 rows x 16 columns and each gets one column's 4 rows.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+template <bool SWAP = false>   // the second and third four of the 16 columns exchanged
 __device__ __forceinline__ u32x2 read_columns(const void *tile, int stride, int row, int column)   // rows row .. row + 3, 16 columns from `column` on, over 16 lanes
 {
-    const int l16 = threadIdx.x & 15;
-    const u16 *at = static_cast<const u16 *>(tile) + (row + (l16 >> 2)) * stride + column + 4 * (l16 & 3);
+    const int l16 = threadIdx.x & 15, four = SWAP ? (l16 & 1) << 1 | (l16 >> 1 & 1) : l16 & 3;
+    const u16 *at = static_cast<const u16 *>(tile) + (row + (l16 >> 2)) * stride + column + 4 * four;
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)const_cast<u16 *>(at)));
 }
 template <typename T> struct Chunk {   // float
@@ -440,7 +442,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     const size_t row0 = (size_t)s.row;
     const float a = g.a[h], bias = g.dt_bias ? g.dt_bias[h] : 0.0f, skip = g.d ? g.d[h] : 0.0f;
 
-    // the state, D-layout: register i of tile nt is n = 32 nt + 8 (i / 4) + 4 half + i % 4 of channel p
+    // the state: register i of tile nt is n = 32 nt + 16 (i / 8) + 8 half + i % 8 of channel p
     f32x16 S[NT];
     const size_t head = (size_t)h * P * N, seg_cells = (size_t)g.heads * P * N;
     const float *start = cut.rows ? (STATE ? nullptr : cut.states + ((size_t)b * cut.count + seg) * seg_cells) : g.state && s.pos > 0 ? g.state + (size_t)s.slot * seg_cells : nullptr;
@@ -452,7 +454,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int n = 32 * nt + 8 * q + 4 * half;
+                const int n = 32 * nt + 16 * (q >> 1) + 8 * half + 4 * (q & 1);
                 if ((N & 3) == 0) {
                     const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(sr, cell(n), 0, 0);
 #pragma unroll
@@ -639,10 +641,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
 #pragma unroll
             for (int kb = 0; kb < 2 * NT; ++kb) {
                 u32x4 cf[TX], bf[TX], sf[K::M];
-                auto frag = [&](const u16 *row) {   // k = 0-3, 8-11 or 4-7, 12-15 of 16
-                    const u32x2 lo = *reinterpret_cast<const u32x2 *>(row + 16 * kb + 4 * half), hi = *reinterpret_cast<const u32x2 *>(row + 16 * kb + 8 + 4 * half);
-                    return (u32x4){lo[0], lo[1], hi[0], hi[1]};
-                };
+                auto frag = [&](const u16 *row) { return *reinterpret_cast<const u32x4 *>(row + 16 * kb + 8 * half); };
 #pragma unroll
                 for (int x = 0; x < TX; ++x) cf[x] = frag(Cs[buf][x][l32]), bf[x] = frag(Bs[buf][x][l32]);
                 float sv[8];
@@ -694,7 +693,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
                     u32x4 bf[TX];
 #pragma unroll
                     for (int x = 0; x < TX; ++x) {
-                        const u32x2 lo = read_columns(&Bs[buf][x][0][0], NS, 16 * kb + 4 * half, 32 * nt + (l32 & 16)), hi = read_columns(&Bs[buf][x][0][0], NS, 16 * kb + 8 + 4 * half, 32 * nt + (l32 & 16));
+                        const u32x2 lo = read_columns<true>(&Bs[buf][x][0][0], NS, 16 * kb + 4 * half, 32 * nt + (l32 & 16)), hi = read_columns<true>(&Bs[buf][x][0][0], NS, 16 * kb + 8 + 4 * half, 32 * nt + (l32 & 16));
                         bf[x] = (u32x4){lo[0], lo[1], hi[0], hi[1]};
                     }
                     product<2>(S[nt], bf, W[kb]);
@@ -762,7 +761,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int n = 32 * nt + 8 * q + 4 * half;
+                const int n = 32 * nt + 16 * (q >> 1) + 8 * half + 4 * (q & 1);
                 u32x4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(S[nt][4 * q + e]);
