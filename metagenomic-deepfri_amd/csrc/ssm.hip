@@ -37,7 +37,7 @@ __device__ __forceinline__ float softplus(float v)
     r = fmaf(q, r, 2.0f / 5.0f);
     r = fmaf(q, r, 2.0f / 3.0f);
     r = fmaf(q, r, 2.0f);
-    return fmaf(s, r, v > 0.0f ? v : 0.0f * v);   // (0 v: a NaN stays one)
+    return fmaf(s, r, v > 0.0f || v != v ? v : 0.0f);   // (a NaN stays one, -infinity gives 0)
 }
 // one value of any of the three types, by code (uniform): the step sizes dt, which are read once per head and row
 __device__ __forceinline__ float load_any(const void *p, size_t i, int dt)
@@ -786,9 +786,20 @@ __global__ __launch_bounds__(256) void k_scan_carry(mdf_scan_args g, ScanSplit c
     float *at = cut.states + (size_t)b * cut.count * cells + i;
     const float *decay = cut.decays + (size_t)b * cut.count * g.heads + h;
     at[0] = v;
-    for (int k = 1; k < segs; ++k) {
-        v = fmaf(__builtin_amdgcn_exp2f(decay[(size_t)(k - 1) * g.heads]), v, at[(size_t)k * cells]);
-        at[(size_t)k * cells] = v;
+    constexpr int AHEAD = 8;   // segments on their way from memory at once
+    for (int k = 1; k < segs; k += AHEAD) {
+        float own[AHEAD], d[AHEAD];
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const int n = min(k + e, segs - 1);
+            own[e] = at[(size_t)n * cells], d[e] = decay[(size_t)(n - 1) * g.heads];
+        }
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            if (k + e >= segs) break;
+            v = fmaf(__builtin_amdgcn_exp2f(d[e]), v, own[e]);
+            at[(size_t)(k + e) * cells] = v;
+        }
     }
 }
 

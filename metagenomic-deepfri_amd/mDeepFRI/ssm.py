@@ -155,7 +155,8 @@ def _indices(t, name: str, device, count: int):
 def _state(t, name: str, device, dtype, tail: tuple):
     if t.dtype != dtype or tuple(t.shape[1:]) != tail or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {('*',) + tail} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+    if t.requires_grad and _torch().is_grad_enabled():
+        raise ValueError(f"{name} asks for a gradient: the state-space operators are inference only")
 
 
 def _check_rows(r: _Rows, rows: SequenceRows, device, total: int, slots, positions, state) -> None:

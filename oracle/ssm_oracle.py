@@ -63,7 +63,7 @@ def scan(x, dt, a, b, c, lengths, row_off, d=None, dt_bias=None, state=None, slo
                 r = row_off[s] + t
                 v = dt[r] + (0 if dt_bias is None else dt_bias)
                 delta = np.maximum(v, 0) + np.log1p(np.exp(-np.abs(v)))
-                rel = 12 + np.abs(v)                      # steps that softplus may be off by
+                rel = 12 + np.minimum(np.abs(v), 200)     # steps that softplus may be off by (it is 0, or v itself, far out)
                 decay = np.exp(delta * a)[:, None, None]
                 new = (delta[:, None] * x[r])[:, :, None] * b[r][rep][:, None, :]
                 h = decay * h + new

@@ -177,6 +177,21 @@ def test_rows_of_no_sequence_do_not_reach_results(dtype, groups, head_dim, state
     assert bool((got[~inside] == 0).all()) and bool((cgot[~inside] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_a_step_size_of_minus_infinity_masks_its_token(dtype):
+    """softplus(-inf) = 0: the token changes no state and reads the one in front of it; the type's lowest value does the same; a row of nothing but such
+    tokens gives d x alone."""
+    rows, x, dt, a, b, c, kw = scan_inputs(24, [70, 40], 3, 1, 32, 48, dtype)
+    dt = dt.clone()
+    dt[5:9, 1], dt[64, 0], dt[70:110, 2] = -math.inf, torch.finfo(dt.dtype).min, -math.inf
+    got, want = check_scan(rows, x, dt, a, b, c, kw)
+    assert torch.isfinite(got).all()
+    near(got[70:, 2], f64(x[70:, 2]) * float(kw["d"][2]), np.abs(f64(x[70:, 2])) * 1e-6 + 1e-30)
+    xbc, sdt, sa, skw = step_inputs(25, 4, 3, 1, 32, 48, 4, dtype)
+    sdt[1] = -math.inf
+    check_step(xbc, sdt, sa, skw)
+
+
 def test_scan_cut_into_segments_skips_sequences_and_spoils_only_what_follows():
     """Sequences longer than a workgroup's share: their segments run side by side and hand their states on.  A skipped one stays as it is, a NaN spoils its
     channel from its token to the sequence's end through every later segment, and the workspace is refused when it is too small."""
