@@ -116,7 +116,9 @@ __device__ __forceinline__ int seq_before(const int32_t *row_off, int B, int64_t
 
 // ---- the short causal convolution ----------------------------------------------------------------------------------------------------------------
 // A thread owns V channels (16 bytes) of `steps` tiles of CONV_ROWS rows.  A tile's rows are requested at once, the width - 1 in front of them are still
-// in registers from the tile before (or requested too), the weights stay in registers.  Bound by memory: each element is read and written once.
+// in registers from the tile before (or requested too), the weights stay in registers.  Bound by memory: each element is read and written once
+// (144 753 rows x 640 in 256 sequences, width 4, bfloat16: 371 MB in 93 us, 4.0 TB/s; SiLU and the conversions are about 17 instructions a value under it).  Tiles of
+// 16 rows or 4 channels a thread measured 100 to 232 us there.
 // Rows take their taps from registers; only a sequence's first width - 1 rows, which look into the kept state or before the sequence, look
 // every tap up.  The tile with a sequence's first row makes all of those rows, wherever they lie, and then keeps the sequence's last inputs:
 // nobody else reads or writes these channels' entries, so a short sequence that overwrites an entry it still needed is no race.
@@ -232,11 +234,12 @@ __global__ __launch_bounds__(256, W <= 3 ? 3 : W <= 7 ? 2 : 1) void k_conv(mdf_c
 // the next product takes them as its k.  For M that order is 0-3, 8-11 | 4-7, 12-15 per 16, and X is read in it; the state's rows are put in such an order by
 // the reads of B^T that its registers are k in their natural order and C is read as it lies.  (B C^T) comes out transposed,
 // lane = i, and so does Y: a lane holds four consecutive channels of a row, which leave in 16-byte stores (with a swap between the halves for 16-bit types).
-// X comes in 16-byte loads through a tile in LDS; it and B^T are read from their rows by the transposing read.  (A value per lane and instruction, 16 loads and
-// 16 stores per chunk, cost 95 of 350 us.)
+// X comes in 16-byte loads through a tile in LDS; it and B^T are read from their rows by the transposing read.
 // Operands are sums of bfloat16 terms: bfloat16 inputs are one, float16 two and float32 three (all exact).  M and S, which only feed rounded outputs, take two
 // terms (2^-16) for the 16-bit types and three for float32; what goes into the state takes three always, so the state is a float32 one for every type.
-// Bound for bfloat16 by issue: per chunk and wave 52 matrix instructions (state_dim 128) and about twice their time of vector instructions.
+// Bound for bfloat16 by issue: per chunk and wave about 780 vector and 52 matrix instructions (state_dim 128), which hardly overlap with two waves per SIMD.  128 sequences
+// of 512 rows, 32 heads of 64 x 128: 315 to 327 us (its bytes would take 113); 257 without the matrix instructions, 287 without splitting S, M and W into terms.
+// Measured there: 8 waves a workgroup 335, three waves per SIMD 590 (spills), matrix and vector instructions woven by hand 346.
 // Long sequences are cut into segments when there are too few (sequence, head) pairs to fill the GPU: a first launch makes each segment's state from zero
 // (STATE: no Y, no C), a small one carries the states from segment to segment, the last one makes Y.
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -251,7 +254,7 @@ __device__ __forceinline__ unsigned cvt_pk_bf16(float a, float b)
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, b2));
 }
 // Two values -> TERMS packed bf16 pairs whose sum they are: each term takes the leading 8 bits of what the ones before leave over (cut off, not rounded:
-// one v_perm for the pair; v_cvt_pk_bf16_f32 takes twice the time), so three terms are exact.  The last of two terms is rounded: 2^-16.
+// one v_perm for the pair), so three terms are exact.  The last of two terms is rounded: 2^-16.
 template <int TERMS>
 __device__ __forceinline__ void split_pair(float a, float b, unsigned (&o)[TERMS])
 {
@@ -407,7 +410,8 @@ struct ScanSplit {          // segments of long sequences; rows == 0: none
     float *decays;          // (B, count, heads): log2 of a segment's whole decay
 };
 
-// WORDS: every row of x, b and c, and every head's and group's part of it, begins on a word
+// WORDS: every row of x, b and c, and every head's and group's part of it, begins on a word.  A template, since the choice inside the loop cost aligned calls 375 us
+// in place of 319 (128 x 512 rows as above); unaligned ones load whole words and shift them.
 template <typename T, int NT, bool STATE, bool WORDS>
 __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2) void k_scan(mdf_scan_args g, ScanSplit cut, int items, int unit_blocks)
 {
@@ -722,8 +726,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             if (k & 1) decays(t0 + SCAN_Q);
             request(t0 + 2 * SCAN_Q);
         }
-        if constexpr (!STATE)
-        if (works) {
+        if (!STATE && works) {
             // ---- a row's channels out: register i is channel p0 + 8 (i / 4) + 4 half + i % 4
             const auto yr = rows_at(yp + (size_t)t0 * yrow, min(SCAN_Q, last - t0), yrow, width);
             const unsigned at = fresh(l32 * yrow + col);
@@ -804,7 +807,7 @@ __global__ __launch_bounds__(256) void k_scan_carry(mdf_scan_args g, ScanSplit c
 }
 
 // ---- one token of many sequences -----------------------------------------------------------------------------------------------------------------------
-// Bound by the states' traffic, 8 bytes per state element; for a few sequences by latency.  A workgroup owns `rows` channels of one head: LN lanes hold a
+// Bound by the states' traffic, 8 bytes per state element (256 sequences of 32 x 64 x 128: 544 MB in 104 us, 5.2 TB/s); for a few sequences by latency.  A workgroup owns `rows` channels of one head: LN lanes hold a
 // channel's state_dim values (V each, J times), 256 / LN channels go at once.  All its state is requested first, then the convolution of its own
 // channels and of the group's B and C is made into LDS (every workgroup of a group makes B and C again: 2 N width products against a state of
 // rows x N), then the state is advanced in registers and stored where it came from.
@@ -882,8 +885,8 @@ __global__ __launch_bounds__(256) void k_step(mdf_step_args g, int rows)
 
 // ---- block norms ------------------------------------------------------------------------------------------------------------------------------------
 // One pass: a row's inputs are requested together, live in registers as f32 through both norms and leave once.  TPR threads per (row, group) hold
-// VPT x 8 values each: a wave holds widths to 2 048 (its sums need no LDS), 256 threads to 8 192, 1 024 to 16 384.  Bound by memory.  Sums: in order
-// over a thread's values, then a tree over lanes -- the same for every row, whatever the batch.
+// VPT x 8 values each; TPR = 64 are four rows per workgroup, whose sums need no LDS.  Bound by memory: 65 536 rows of 2 048 with a gate in bfloat16 (805 MB) take
+// 150 us, 5.4 TB/s.  Sums: in order over a thread's values, then a tree over lanes -- the same for every row, whatever the batch.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float *part)
 {
@@ -902,11 +905,11 @@ __device__ __forceinline__ float row_sum(float v, float *part)
 
 // thread t of a row holds the 8 values from (v TPR + t) 8 on; a row's last few are taken one by one
 template <typename T, typename R, int TPR, int VPT>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_block_norm(mdf_block_norm_args g)
+__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_block_norm(mdf_block_norm_args g)
 {
     __shared__ float part[16];
     const int t = threadIdx.x % TPR, width = g.dim / g.groups, c0 = blockIdx.y * width;
-    const size_t row = TPR < 256 ? (size_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : blockIdx.x;
+    const size_t row = TPR == 64 ? (size_t)blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x;
     if (row >= (size_t)g.rows) return;    // whole waves (TPR = 64) only
     const T *s = static_cast<const T *>(g.s) + row * g.lds + c0, *gate = static_cast<const T *>(g.gate) + row * g.ldg + c0;
     const R *res = static_cast<const R *>(g.residual) + row * g.ldr + c0;
@@ -1086,18 +1089,21 @@ static bool overlap(const void *p, int64_t ldp, int64_t wp, size_t ep, const voi
 template <typename T, typename R, int TPR, int VPT>
 static void norm_launch(const mdf_block_norm_args &a, hipStream_t st)
 {
-    const dim3 grid((unsigned)(TPR < 256 ? (a.rows + 256 / TPR - 1) / (256 / TPR) : a.rows), a.groups), block(TPR < 256 ? 256 : TPR);
+    const dim3 grid((unsigned)(TPR == 64 ? (a.rows + 3) / 4 : a.rows), a.groups), block(TPR == 64 ? 256 : TPR);
     hipLaunchKernelGGL((k_block_norm<T, R, TPR, VPT>), grid, block, 0, st, a);
 }
+// As few threads as hold the row in one vector each, to 512 of them; then two vectors.  128 Mi bfloat16 values in rows of `width` with a gate, us:
+//   512: 64 threads x 1 vector 145-158, 128 x 1 231-246        1 024: 128 x 1 144, 64 x 2 166, 256 x 1 233       2 048: 256 x 1 143, 128 x 2 160, 64 x 4 311, 512 x 1 255
+//   4 096: 512 x 1 152, 256 x 2 188, 1 024 x 1 383             8 192: 512 x 2 200, 1 024 x 1 228, 256 x 4 301    16 384: 1 024 x 2 210, the walk 500
 template <typename T, typename R>
 static void norm_by_width(const mdf_block_norm_args &a, hipStream_t st)
 {
     const int width = a.dim / a.groups;
     if (width <= 512) norm_launch<T, R, 64, 1>(a, st);
-    else if (width <= 1024) norm_launch<T, R, 64, 2>(a, st);
+    else if (width <= 1024) norm_launch<T, R, 128, 1>(a, st);
     else if (width <= 2048) norm_launch<T, R, 256, 1>(a, st);
-    else if (width <= 4096) norm_launch<T, R, 256, 2>(a, st);
-    else if (width <= 8192) norm_launch<T, R, 1024, 1>(a, st);
+    else if (width <= 4096) norm_launch<T, R, 512, 1>(a, st);
+    else if (width <= 8192) norm_launch<T, R, 512, 2>(a, st);
     else if (width <= 16384) norm_launch<T, R, 1024, 2>(a, st);
     else hipLaunchKernelGGL((k_block_norm_walk<T, R>), dim3((unsigned)a.rows, a.groups), dim3(256), 0, st, a);
 }
@@ -1170,9 +1176,11 @@ static void step_launch(const mdf_step_args &a, hipStream_t st)
     const bool wide = N % 4 == 0;   // else one value at a time
     const int ln = wide ? (N <= 16 ? 4 : N <= 32 ? 8 : N <= 64 ? 16 : 32) : N <= 16 ? 16 : N <= 32 ? 32 : 64;
     const int per = 256 / ln;
-    // channels per workgroup: as many as a thread's registers hold (8 x `per`) while that leaves four workgroups per CU, fewer for few sequences
+    // Channels per workgroup: as many as a thread's registers hold (8 x `per`) while that leaves two workgroups per CU, fewer for few sequences: each workgroup makes
+    // B and C again.  32 heads of 64 channels x 128, us with 8 / 16 / 32 / 64 channels: 2 sequences 4.9 / 4.9 / 5.5 / 6.5, 4: 6.3 / 5.4 / 5.8 / 6.8,
+    // 8: 10.1 / 7.2 / 6.4 / 7.3, 16: 15.8 / 11.1 / 8.8 / 8.3, 128: 95 / 59 / 51 / 45.
     int rows = std::min(a.head_dim, 8 * per);
-    while (rows > per && (int64_t)a.B * a.heads * ((a.head_dim + rows - 1) / rows) < 1024) rows = std::max(per, (rows / 2 + per - 1) / per * per);
+    while (rows > per && (int64_t)a.B * a.heads * ((a.head_dim + rows - 1) / rows) < 512) rows = std::max(per, (rows / 2 + per - 1) / per * per);
     const dim3 grid((unsigned)a.B, a.heads, (a.head_dim + rows - 1) / rows);
 #define MDF_S(ln_, v_, j_) hipLaunchKernelGGL((k_step<T, ln_, v_, j_>), grid, dim3(256), 0, st, a, rows)
     if (wide) {
@@ -1235,10 +1243,15 @@ int mdf_causal_conv_dev(const mdf_conv_args *a, void *stream)
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int v = a->channels >= 16 / (int)e ? 16 / (int)e : 1;
     const int lanes = (a->channels + v - 1) / v;
-    // tiles per thread: the weights cost 4 (width + 1) bytes per channel and thread, so as many as leave the GPU 4 waves per SIMD to run (256 x 4 x 4)
-    const int64_t tiles = (a->rows.R + CONV_ROWS - 1) / CONV_ROWS;
+    // Tiles per thread: further ones save the weights, the rows in front and a search, and cost parallel threads; they pay once one tile each is more than
+    // the waves that are resident at once.  1 / 2 / 4 tiles, us (640 channels; threads of one tile in units of 65 536, one wave per SIMD):
+    //   bf16  1.7 units: width 4 15.0 / 16.8 / 21.3, 8 22.8 / 28.1 / 34.7      3.3: width 2 16.9 / 17.8 / 18.1, 4 23.3 / 21.1 / 21.9, 8 38.6 / 29.2 / 30.3
+    //         5.3: width 4 30.6 / 26.3 / 28.6, 5 37.1 / 32.5 / 30.8            21: width 2 71.8 / 73.2 / 78.6, 4 101 / 84.5 / 84.8, 8 169 / 138 / 111
+    //   f32   3.3: width 4 15.3 / 15.8 / 16.7                                  6.6: width 2 21.1 / 20.4 / 19.8, 4 24.0 / 22.7 / 21.6, 8 41.3 / 35.0 / 27.0
+    const int64_t tiles = (a->rows.R + CONV_ROWS - 1) / CONV_ROWS, units = tiles * lanes / 65536;
     int steps = 1;
-    while (steps < 4 && tiles * lanes >= (int64_t)2 * steps * 64 * 4096) steps *= 2;
+    if (e == 4) steps = units >= 6 ? 4 : 1;
+    else if (a->width > 2 && units >= 3) steps = a->width > 4 && units >= 5 ? 4 : 2;
     const int64_t threads = (tiles + steps - 1) / steps * lanes;
     MDF_REQUIRE((threads + 255) / 256 < (int64_t)1 << 31, "causal_conv_dev: %lld rows of %d channels are too many", (long long)a->rows.R, a->channels);
     const dim3 grid((unsigned)((threads + 255) / 256));
