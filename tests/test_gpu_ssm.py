@@ -84,6 +84,15 @@ def test_conv_keeps_its_state(dtype, lens, channels, width):
     check_conv(rows, x, weight, bias, kw)
 
 
+@pytest.mark.parametrize("dtype, width, total", [("f32", 3, 12400), ("f32", 8, 12400), ("bf16", 4, 12400), ("f16", 7, 20600), ("bf16", 2, 12400)])
+def test_conv_of_many_rows_takes_several_tiles_per_thread(dtype, width, total):
+    """Sequences that begin and end anywhere in a thread's tiles, some shorter than the kernel is wide, with their states."""
+    some = np.random.default_rng(5).choice([0, 1, 2, 3, 7, 8, 9, 31, 70, 500], size=2000)
+    lens = some[: int(np.searchsorted(np.cumsum(some), total)) + 1].tolist()
+    rows, x, weight, bias, kw = conv_inputs(5, lens, 1024, width, dtype, kept=True)
+    check_conv(rows, x, weight, bias, kw)
+
+
 def test_conv_skips_sequences_and_leaves_other_rows():
     rows, x, weight, bias, kw = conv_inputs(3, [5, 20, 7, 40], 64, 4, "bf16", align=16, kept=True)
     kw["slots"] = torch.tensor([1, -1, 99, 0], dtype=torch.int32, device="cuda")
@@ -393,6 +402,15 @@ def test_norm_forms(dtype, rows, dim):
             ("f32", True, False, "silu", False, False, False, False), (None, True, False, "silu", True, True, False, False)]):
         s, kw = norm_inputs(31 + i, rows, dim, dtype, residual, gate, post, pre, center, vec)
         check_norm(s, dict(kw, gate_first=first, gate_act=act))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim", [512, 520, 1025, 2049, 4096, 4097, 8192, 8193, 16384, 16385])
+def test_norm_widths(dtype, dim):
+    """The widths on both sides of each change of threads per row."""
+    for i, (residual, gate, post, pre, center, vec) in enumerate([(None, True, True, False, False, False), ("f32", True, True, True, True, True), ("same", False, True, True, False, False)]):
+        s, kw = norm_inputs(61 + i, 3, dim, dtype, residual, gate, post, pre, center, vec)
+        check_norm(s, dict(kw, gate_first=i == 0))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
