@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256, W <= 3 ? 3 : W <= 7 ? 2 : 1) void k_conv(mdf_c
 // Operands are sums of bfloat16 terms: bfloat16 inputs are one, float16 two and float32 three (all exact).  M and S, which only feed rounded outputs, take two
 // terms (2^-16) for the 16-bit types and three for float32; what goes into the state takes three always, so the state is a float32 one for every type.
 // Bound for bfloat16 by issue: per chunk and wave about 780 vector and 52 matrix instructions (state_dim 128), which hardly overlap with two waves per SIMD.  128 sequences
-// of 512 rows, 32 heads of 64 x 128: 315 to 327 us (its bytes would take 113); 257 without the matrix instructions, 287 without splitting S, M and W into terms.
+// of 512 rows, 32 heads of 64 x 128: 300 to 327 us from card to card (its bytes would take 113); 257 without the matrix instructions, 287 without splitting S, M and W into terms.
 // Measured there: 8 waves a workgroup 335, three waves per SIMD 590 (spills), matrix and vector instructions woven by hand 346.
 // Long sequences are cut into segments when there are too few (sequence, head) pairs to fill the GPU: a first launch makes each segment's state from zero
 // (STATE: no Y, no C), a small one carries the states from segment to segment, the last one makes Y.
