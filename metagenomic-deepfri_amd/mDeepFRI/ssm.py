@@ -265,7 +265,8 @@ def selective_scan(x, dt, a, b, c, rows: SequenceRows, *, d=None, dt_bias=None, 
 
     x and the result (R, heads, head_dim), dt (R, heads), b and c (R, groups, state_dim) -- views into one wider array are fine, only the
     row strides are free; a, d, dt_bias (heads) f32.  head_dim 1..256, state_dim 1..128, heads a multiple of groups.  state (n_slots, heads,
-    head_dim, state_dim) f32 is continued where positions > 0 and left behind for the next call; slots / positions as in causal_conv."""
+    head_dim, state_dim) f32 is continued where positions > 0 and left behind for the next call; slots / positions as in causal_conv.
+    dt = -infinity masks a token: the state passes it unchanged (y still holds H c + d x)."""
     device = x.device
 
     def check():
