@@ -235,8 +235,9 @@ __global__ __launch_bounds__(256, W <= 3 ? 3 : W <= 7 ? 2 : 1) void k_conv(mdf_c
 // the reads of B^T that its registers are k in their natural order and C is read as it lies.  (B C^T) comes out transposed,
 // lane = i, and so does Y: a lane holds four consecutive channels of a row, which leave in 16-byte stores (with a swap between the halves for 16-bit types).
 // X comes in 16-byte loads through a tile in LDS; it and B^T are read from their rows by the transposing read.
-// Operands are sums of bfloat16 terms: bfloat16 inputs are one, float16 two and float32 three (all exact).  M and S, which only feed rounded outputs, take two
-// terms (2^-16) for the 16-bit types and three for float32; what goes into the state takes three always, so the state is a float32 one for every type.
+// Operands are sums of bfloat16 terms: bfloat16 inputs are one, float16 two and float32, M, S and what goes into the state three (all exact); of two such sums the
+// term products below 2^-24 are left out.  So for every type the arithmetic is that of float32, and a 16-bit output is rounded once.  (M and S in two terms, 2^-16,
+// took 324 us in place of 360 in the case below, and left its bfloat16 outputs 1.2e-4 in the 2-norm off float32 products rounded once; now 2.3e-5.)
 // Bound for bfloat16 by issue: per chunk and wave about 780 vector and 52 matrix instructions (state_dim 128), which hardly overlap with two waves per SIMD.  128 sequences
 // of 512 rows, 32 heads of 64 x 128: 300 to 327 us from card to card (its bytes would take 113); 257 without the matrix instructions, 287 without splitting S, M and W into terms.
 // Measured there: 8 waves a workgroup 335, three waves per SIMD 590 (spills), matrix and vector instructions woven by hand 346.
@@ -254,16 +255,12 @@ __device__ __forceinline__ unsigned cvt_pk_bf16(float a, float b)
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, b2));
 }
 // Two values -> TERMS packed bf16 pairs whose sum they are: each term takes the leading 8 bits of what the ones before leave over (cut off, not rounded:
-// one v_perm for the pair), so three terms are exact.  The last of two terms is rounded: 2^-16.
+// one v_perm for the pair), so three terms are exact for float32, two for float16.
 template <int TERMS>
 __device__ __forceinline__ void split_pair(float a, float b, unsigned (&o)[TERMS])
 {
 #pragma unroll
     for (int i = 0; i < TERMS; ++i) {
-        if (TERMS == 2 && i == 1) {
-            o[i] = cvt_pk_bf16(a, b);
-            continue;
-        }
         o[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);   // the upper halves
         if (i + 1 < TERMS) {
             a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
@@ -363,10 +360,11 @@ __device__ __forceinline__ bool any_odd(const Raw<T, 8> &r)
     return max(most[0], most[1]) >= (std::is_same<T, Bf16>::value ? 0x7f80 : 0x7c00);
 }
 
+// terms of an input, and the largest i + j of the term products of two inputs (float16: all four)
 template <typename T> struct Terms;
-template <> struct Terms<Bf16> { static constexpr int X = 1, IN = 0, M = 2, OUT = 1; };   // terms of an input, cutoff of input x input; terms of M and S, cutoff of M x X and C x S
-template <> struct Terms<F16> { static constexpr int X = 2, IN = 1, M = 2, OUT = 1; };
-template <> struct Terms<float> { static constexpr int X = 3, IN = 2, M = 3, OUT = 2; };
+template <> struct Terms<Bf16> { static constexpr int X = 1, IN = 0; };
+template <> struct Terms<F16> { static constexpr int X = 2, IN = 2; };
+template <> struct Terms<float> { static constexpr int X = 3, IN = 2; };
 
 constexpr int SCAN_Q = 32, SCAN_WAVES = 4;
 
@@ -644,16 +642,16 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             f32x16 G = {};
 #pragma unroll
             for (int kb = 0; kb < 2 * NT; ++kb) {
-                u32x4 cf[TX], bf[TX], sf[K::M];
+                u32x4 cf[TX], bf[TX], sf[3];
                 auto frag = [&](const u16 *row) { return *reinterpret_cast<const u32x4 *>(row + 16 * kb + 8 * half); };
 #pragma unroll
                 for (int x = 0; x < TX; ++x) cf[x] = frag(Cs[buf][x][l32]), bf[x] = frag(Bs[buf][x][l32]);
                 float sv[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sv[e] = S[kb / 2][8 * (kb & 1) + e];
-                split8<K::M>(sv, sf);
+                split8<3>(sv, sf);
                 product<K::IN>(G, bf, cf);     // lane = row i of C, registers = j
-                product<K::OUT>(Y, sf, cf);    // lane = row i, registers = channels
+                product<2>(Y, sf, cf);    // lane = row i, registers = channels
             }
             // ---- M, and what it adds
             float m[16];
@@ -671,9 +669,9 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             }
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                u32x4 mf[K::M];
-                split8<K::M>(m + 8 * kb, mf);
-                product<K::OUT>(Y, X[kb], mf);
+                u32x4 mf[3];
+                split8<3>(m + 8 * kb, mf);
+                product<2>(Y, X[kb], mf);
             }
         }
         // ---- the state

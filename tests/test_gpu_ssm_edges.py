@@ -1,0 +1,41 @@
+"""The state-space block's operators on the GPU in calls at the edges of what their documentation allows."""
+import numpy as np
+import pytest
+
+import ssm_oracle as orc
+from test_gpu_ssm import TYPES, f64, scan_inputs, ssm
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# 16-bit outputs are float32 results, rounded once
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_scan_reads_a_state_to_its_last_bit(dtype):
+    """Masked tokens (D = 0) whose c picks one entry of the state: y is that float32 number, rounded once to the output's type -- no arithmetic in between is
+    inexact, so every bit counts."""
+    heads, head_dim, state_dim, n = 4, 64, 32, 3
+    rows, x, dt, a, b, c, _ = scan_inputs(201, [state_dim] * n, heads, 1, head_dim, state_dim, dtype)
+    g = torch.Generator(device="cuda").manual_seed(202)
+    state = torch.randn(n, heads, head_dim, state_dim, generator=g, device="cuda")
+    c = torch.eye(state_dim, device="cuda").repeat(n, 1).to(x.dtype).unsqueeze(1).contiguous()
+    positions = torch.ones(n, dtype=torch.int32, device="cuda")
+    got = ssm().selective_scan(x, torch.full_like(dt, -np.inf), a, b, c, rows, state=state, positions=positions)
+    want = state.permute(0, 3, 1, 2).reshape(got.shape).to(x.dtype)
+    assert torch.equal(got, want), int((got != want).sum())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lens, state_dim", [([1] * 300, 2), ([1, 3, 2, 4] * 60, 4)])
+def test_scan_rounds_as_float32_arithmetic_does(dtype, lens, state_dim):
+    """Where the oracle's value less and plus its bound of float32 arithmetic round to the same number, every float32 result in between does: the output is that
+    number."""
+    rows, x, dt, a, b, c, kw = scan_inputs(203, lens, 4, 1, 64, state_dim, dtype)
+    want, slack, _ = orc.scan(f64(x), f64(dt), f64(a), f64(b), f64(c), rows.lengths.cpu().numpy(), rows.row_off.cpu().numpy(), d=f64(kw["d"]), dt_bias=f64(kw["dt_bias"]))
+    got = ssm().selective_scan(x, dt, a, b, c, rows, **kw).cpu()
+    low, high = (torch.from_numpy(v).to(TYPES[dtype]) for v in (want - slack, want + slack))
+    told = low == high
+    assert float(told.double().mean()) > 0.9
+    assert torch.equal(got[told], low[told]), int((got[told] != low[told]).sum())
