@@ -73,11 +73,12 @@ def _dtype(t, name: str) -> int:
 
 class SequenceRows:
     """Which rows belong to which sequence: `lengths` (B) and `row_off` (B+1), int32 device tensors, row_off ascending, and the longest length.
-    `dense`: the sequences cover every row (an output made here then needs no zeros).  `build` makes one from host lengths and checks them."""
+    `dense`: the caller's word that the sequences leave out no row of the first `total` (None: of any array that they are used with), whose outputs then need no
+    zeros when they are made here.  `build` makes one from host lengths, checks them and knows both."""
 
-    __slots__ = ("lengths", "row_off", "max_len", "dense", "count", "form")
+    __slots__ = ("lengths", "row_off", "max_len", "dense", "total", "count", "form")
 
-    def __init__(self, lengths, row_off, max_len: int, dense: bool = False):
+    def __init__(self, lengths, row_off, max_len: int, dense: bool = False, total: int | None = None):
         torch = _torch()
         if lengths.dtype != torch.int32 or row_off.dtype != torch.int32 or lengths.dim() != 1 or row_off.dim() != 1 or not lengths.is_contiguous() or not row_off.is_contiguous():
             raise ValueError("lengths and row_off must be contiguous one-dimensional int32 tensors")
@@ -85,7 +86,7 @@ class SequenceRows:
             raise ValueError(f"row_off has {row_off.shape[0]} entries for {lengths.shape[0]} sequences (one more is wanted)")
         if lengths.device != row_off.device or max_len < 0:
             raise ValueError("lengths and row_off lie on different devices, or max_len is negative")
-        self.lengths, self.row_off, self.max_len, self.dense, self.count = lengths, row_off, int(max_len), dense, lengths.shape[0]
+        self.lengths, self.row_off, self.max_len, self.dense, self.total, self.count = lengths, row_off, int(max_len), dense, total, lengths.shape[0]
         self.form = (self.count, lengths.get_device())
 
     @classmethod
@@ -99,7 +100,7 @@ class SequenceRows:
         np.cumsum(-(-n // align) * align, out=off[1:])
         if off[-1] >= 2**31:
             raise ValueError("too many rows for int32 offsets; split the batch")
-        return cls(torch.from_numpy(n.astype(np.int32)).to(device), torch.from_numpy(off.astype(np.int32)).to(device), int(n.max(initial=0)), dense=bool(off[-1] == n.sum()))
+        return cls(torch.from_numpy(n.astype(np.int32)).to(device), torch.from_numpy(off.astype(np.int32)).to(device), int(n.max(initial=0)), dense=bool(off[-1] == n.sum()), total=int(off[-1]))
 
 
 def check_slots(slots, n_slots: int, device="cuda"):
@@ -203,10 +204,10 @@ def _grad() -> bool:
 
 
 def _made(out, like, rows: SequenceRows, shape):
-    """(`zero_skipped` is set for an output made here, so a dense one needs no zeros)"""
+    """(`zero_skipped` is set for an output made here, so one whose every row is a sequence's needs no zeros)"""
     if out is not None:
         return out
-    return like.new_empty(shape) if rows.dense else like.new_zeros(shape)
+    return like.new_empty(shape) if rows.dense and rows.total in (None, shape[0]) else like.new_zeros(shape)
 
 
 def _check_out(out, like) -> None:

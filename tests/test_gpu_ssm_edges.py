@@ -39,3 +39,23 @@ def test_scan_rounds_as_float32_arithmetic_does(dtype, lens, state_dim):
     told = low == high
     assert float(told.double().mean()) > 0.9
     assert torch.equal(got[told], low[told]), int((got[told] != low[told]).sum())
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# rows of no sequence
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens, longer", [([5, 40, 1], 100), ([7], 1), ([], 33), ([0, 0], 5)])
+def test_rows_behind_the_last_sequence_are_zero_in_an_output_made_here(dtype, lens, longer):
+    """An array longer than the sequences in it (a buffer of one size for every batch), while the allocator hands out memory full of NaN."""
+    total = sum(lens) + longer
+    _, x, dt, a, b, c, kw = scan_inputs(211, [total], 3, 1, 32, 48, dtype)
+    rows = ssm().SequenceRows.build(lens)
+    assert rows.dense
+    weight = torch.ones(4, 96, device="cuda")
+    for call in (lambda: ssm().selective_scan(x, dt, a, b, c, rows, **kw), lambda: ssm().causal_conv(x.flatten(1), weight, rows).view(x.shape)):
+        junk = torch.full(x.shape, np.nan, dtype=x.dtype, device="cuda")
+        del junk
+        got = call()
+        assert bool((got[sum(lens):] == 0).all()) and bool(torch.isfinite(got).all())
+        assert sum(lens) == 0 or bool((got[:sum(lens)] != 0).any())
