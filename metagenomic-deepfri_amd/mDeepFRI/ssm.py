@@ -16,6 +16,7 @@ inputs, everything in between is f32."""
 from __future__ import annotations
 
 import ctypes
+import operator
 import struct
 from ctypes import c_float, c_int32, c_int64, c_void_p
 
@@ -195,6 +196,13 @@ def _known(entry: int, form, check):
     return tail
 
 
+def _number(v, name: str, kind=lambda v: c_float(v).value):
+    """A number of the host as it is now, in float32; one that lies on a GPU would have to be waited for."""
+    if getattr(v, "is_cuda", False):
+        raise ValueError(f"{name} is a tensor on {v.device}: a number on the host is wanted (nothing here waits for the GPU)")
+    return kind(v)
+
+
 def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -230,6 +238,7 @@ def _call(fn, device, *args) -> None:
 
 _ROWS = "4Qqiii4x"                                 # mdf_seq_rows
 _CONV, _SCAN, _STEP, _NORM = (struct.Struct(f) for f in (_ROWS + "5Q", _ROWS + "9Q", "12Q", "10Q"))   # up to the last address of each structure
+_SCALES = struct.Struct("2f4x")                    # mdf_block_norm_args' end: values, so packed at every call like the addresses
 
 
 def causal_conv(x, weight, rows: SequenceRows, *, bias=None, silu: bool = True, state=None, slots=None, positions=None, out=None):
@@ -351,10 +360,11 @@ def block_norm(s, *, residual=None, gate=None, gate_act: str = "silu", gate_firs
         r = residual + scale * scale_vec * v  where a residual is given;  out = pre(r) where pre_weight is given
 
     Returns (r or None, out or None); without a residual out is v, or pre(v).  post / pre: x / sqrt(mean(x^2) + eps) * weight + bias, of x less its
-    mean with `center`; post on each of `groups` equal parts of a row.  s and gate share a type; the residual is float32 or of that type, and r has
-    its type.  residual_out may be the residual itself, out may be s or the gate."""
+    mean with `center`; post on each of `groups` equal parts of a row.  scale, eps and groups are numbers on the host.  s and gate share a type; the residual
+    is float32 or of that type, and r has its type.  residual_out may be the residual itself, out may be s or the gate."""
     device = s.device
     has_out = pre_weight is not None or residual is None
+    scale, eps, groups = _number(scale, "scale"), _number(eps, "eps"), _number(groups, "groups", operator.index)
 
     def check():
         if s.dim() != 2:
@@ -382,15 +392,16 @@ def block_norm(s, *, residual=None, gate=None, gate_act: str = "silu", gate_firs
             raise ValueError("out without a pre-norm beside a residual: there is nothing to write there")
         _check_out(out, s)
         g.ldo = dim if out is None else _matrix(out, "out", device, (dim,), rows)
-        g.rows, g.dim, g.groups, g.gate_act, g.gate_first, g.center, g.scale, g.eps = rows, dim, groups, ACTS[gate_act], bool(gate_first), bool(center), scale, eps
-        return bytes(g)[_NORM.size:]
+        g.rows, g.dim, g.groups, g.gate_act, g.gate_first, g.center = rows, dim, groups, ACTS[gate_act], bool(gate_first), bool(center)
+        return bytes(g)[_NORM.size:_Norm.scale.offset]
 
-    tail = _known(3, (_form(s), _form(residual), _form(gate), gate_act, bool(gate_first), _flat(post_weight), _flat(post_bias), groups, scale, _flat(scale_vec), _flat(pre_weight),
-                      _flat(pre_bias), eps, bool(center), _form(residual_out), _form(out), _grad()), check)
+    tail = _known(3, (_form(s), _form(residual), _form(gate), gate_act, bool(gate_first), _flat(post_weight), _flat(post_bias), groups, _flat(scale_vec), _flat(pre_weight),
+                      _flat(pre_bias), bool(center), _form(residual_out), _form(out), _grad()), check)
     if residual_out is None and residual is not None:
         residual_out = residual.new_empty(s.shape)
     if out is None and has_out:
         out = s.new_empty(s.shape)
     _call(_hip.lib().mdf_block_norm_dev, device,
-          _NORM.pack(s.data_ptr(), _ptr(gate), _ptr(residual), _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias), _ptr(scale_vec), _ptr(residual_out), _ptr(out)) + tail)
+          _NORM.pack(s.data_ptr(), _ptr(gate), _ptr(residual), _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias), _ptr(scale_vec), _ptr(residual_out), _ptr(out)) + tail
+          + _SCALES.pack(scale, eps))
     return residual_out, out

@@ -59,3 +59,14 @@ def test_rows_behind_the_last_sequence_are_zero_in_an_output_made_here(dtype, le
         got = call()
         assert bool((got[sum(lens):] == 0).all()) and bool(torch.isfinite(got).all())
         assert sum(lens) == 0 or bool((got[:sum(lens)] != 0).any())
+
+
+def test_a_residual_scale_changed_in_place_is_the_one_used():
+    s, r = torch.ones(3, 64, device="cuda"), torch.zeros(3, 64, device="cuda")
+    scale = torch.tensor(0.5)
+    for k in (0.5, 0.25, -3.0):
+        scale.fill_(k)
+        got, _ = ssm().block_norm(s, residual=r, scale=scale)
+        assert bool((got == k).all())
+    with pytest.raises(ValueError, match="host"):
+        ssm().block_norm(s, residual=r, scale=scale.cuda())
