@@ -402,11 +402,15 @@ __device__ __forceinline__ void buffer_store(float v, __amdgpu_buffer_rsrc_t r, 
 __device__ __forceinline__ void buffer_store(Bf16 v, __amdgpu_buffer_rsrc_t r, unsigned at) { __builtin_amdgcn_raw_buffer_store_b16(v.v, r, at, 0, 0); }
 __device__ __forceinline__ void buffer_store(F16 v, __amdgpu_buffer_rsrc_t r, unsigned at) { __builtin_amdgcn_raw_buffer_store_b16(v.v, r, at, 0, 0); }
 
-struct ScanSplit {          // segments of long sequences; rows == 0: none
-    int rows, count;        // rows per segment (multiple of 64), segments per sequence (at most)
-    float *states;          // (B, count, heads, head_dim, state_dim): a segment's own end state, then its start state
-    float *decays;          // (B, count, heads): log2 of a segment's whole decay
+// Segments of long sequences; rows == 0: none.  A sequence of more than `rows` rows has a slot per segment, from number row / (rows / 2) on, `row` its first:
+// its n segments span more than n - 1 times `rows`, so twice as many halves as it has whole segments, no fewer than n, lie in front of the next sequence's first slot.
+// So 2 R / rows slots do for any mix of lengths (a shorter sequence has none), and a slot's owner is the last sequence whose slots would begin at or before it.
+struct ScanSplit {
+    int rows, slots;        // rows per segment (multiple of 64)
+    float *states;          // (slots, heads, head_dim, state_dim): a segment's own end state, then its start state
+    float *decays;          // (slots, heads): log2 of a segment's whole decay
 };
+__device__ __forceinline__ int slot_owner(const mdf_seq_rows &r, const ScanSplit &cut, int slot) { return seq_before(r.row_off, r.B, (int64_t)(slot + 1) * (cut.rows / 2) - 1); }
 
 // WORDS: every row of x, b and c, and every head's and group's part of it, begins on a word.  A template, since the choice inside the loop cost aligned calls 375 us
 // in place of 319 (128 x 512 rows as above); unaligned ones load whole words and shift them.
@@ -421,19 +425,24 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     // Block -> (item, channels): workgroups of one item (which read the same B and C) lie on one XCD -- block b runs on XCD b mod 8 -- and close in time.
     const int xcd = blockIdx.x & 7, place = blockIdx.x >> 3, item = (place / unit_blocks) * 8 + xcd, ub = place % unit_blocks;
     if (item >= items) return;
-    const int b = cut.rows ? item / cut.count : item, seg = cut.rows ? item % cut.count : 0;
+    // items: the slots of segments, then the sequences that are not cut
+    const int b = item >= cut.slots ? item - cut.slots : __builtin_amdgcn_readfirstlane(slot_owner(g.rows, cut, item));
+    if (b < 0) return;
     Seq s = seq_of(g.rows, b, g.state != nullptr);
     s.row = __builtin_amdgcn_readfirstlane((int)s.row), s.count = __builtin_amdgcn_readfirstlane(s.count);   // the same in every lane: addresses by the scalar unit
-    const int first = cut.rows ? seg * cut.rows : 0;
-    if (!STATE && s.count < 0 && seg == 0 && g.zero_skipped) {
+    const bool split = cut.rows && s.count > cut.rows;
+    const int slot0 = split ? (int)s.row / (cut.rows / 2) : 0, seg = split ? item - slot0 : 0;
+    if (split != (item < cut.slots) || seg < 0 || (split && (int64_t)seg * cut.rows >= s.count)) return;   // another item's sequence, or a slot that no segment has
+    const int first = split ? seg * cut.rows : 0;
+    if (!STATE && s.count < 0 && g.zero_skipped) {
         const int r = g.heads / g.groups, pblocks = (g.head_dim + 31) / 32, per_group = (r * pblocks + SCAN_WAVES - 1) / SCAN_WAVES, h0 = ub / per_group * r;
         const int u0 = ub % per_group * SCAN_WAVES, u1 = min(u0 + SCAN_WAVES, r * pblocks) - 1;   // the workgroup's channels lie side by side
         const int c0 = (h0 + u0 / pblocks) * g.head_dim + u0 % pblocks * 32, c1 = (h0 + u1 / pblocks) * g.head_dim + min(u1 % pblocks * 32 + 32, g.head_dim);
         for (int t = 0; t < s.rows; ++t)
             for (int c = c0 + threadIdx.x; c < c1; c += 64 * SCAN_WAVES) static_cast<T *>(g.y)[(size_t)(s.row + t) * g.ldy + c] = from_f32<T>(0.0f);
     }
-    if (s.count <= first) return;                                     // skipped, without rows, or a segment the sequence does not reach
-    const int last = cut.rows && seg + 1 < cut.count ? min(first + cut.rows, s.count) : s.count;
+    if (s.count <= 0) return;                                         // skipped, or without rows
+    const int last = split ? (int)min((int64_t)first + cut.rows, (int64_t)s.count) : s.count;
     if (STATE && last == s.count) return;                              // nobody starts from this segment's end
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
     const int N = g.state_dim, P = g.head_dim, r = g.heads / g.groups, pblocks = (P + 31) / 32, per_group = (r * pblocks + SCAN_WAVES - 1) / SCAN_WAVES;
@@ -447,8 +456,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     // the state: register i of tile nt is n = 32 nt + 16 (i / 8) + 8 half + i % 8 of channel p
     f32x16 S[NT];
     const size_t head = (size_t)h * P * N, seg_cells = (size_t)g.heads * P * N;
-    const float *start = cut.rows ? (STATE ? nullptr : cut.states + ((size_t)b * cut.count + seg) * seg_cells) : g.state && s.pos > 0 ? g.state + (size_t)s.slot * seg_cells : nullptr;
-    float *end = STATE ? cut.states + ((size_t)b * cut.count + seg + 1) * seg_cells : g.state && last == s.count ? g.state + (size_t)s.slot * seg_cells : nullptr;
+    const float *start = split ? (STATE ? nullptr : cut.states + (size_t)(slot0 + seg) * seg_cells) : g.state && s.pos > 0 ? g.state + (size_t)s.slot * seg_cells : nullptr;
+    float *end = STATE ? cut.states + (size_t)(slot0 + seg + 1) * seg_cells : g.state && last == s.count ? g.state + (size_t)s.slot * seg_cells : nullptr;
     auto cell = [&](int n) { return mine && n < N ? fresh((unsigned)(p * N) * 4u) + 4u * n : OUTSIDE; };   // inside the head's state
     if (start && works) {
         const auto sr = rows_at(start + head, 1, 0, (unsigned)(P * N) * 4u);
@@ -772,34 +781,38 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
                     for (int e = 0; e < 4; ++e) __builtin_amdgcn_raw_buffer_store_b32(v[e], sr, cell(n + e), 0, 0);
             }
     }
-    if (STATE && works && lane == 0) cut.decays[((size_t)b * cut.count + seg) * g.heads + h] = (float)total;   // several waves of a head store the same value
+    if (STATE && works && lane == 0) cut.decays[(size_t)(slot0 + seg) * g.heads + h] = (float)total;   // several waves of a head store the same value
 }
 
-// The states from segment to segment: a thread per state value; what a segment made from zero becomes what the next one starts from.
+// The states from segment to segment: a thread per state value (or a few); what a segment made from zero becomes what the next one starts from.  blockIdx.y: a
+// sequence, or, where there are more of them, a multiple of `rows`, for the sequence whose first one that is (one that is cut has such a row).
 __global__ __launch_bounds__(256) void k_scan_carry(mdf_scan_args g, ScanSplit cut)
 {
-    const int b = blockIdx.y;
+    const int b = gridDim.y == (unsigned)g.rows.B ? (int)blockIdx.y : seq_before(g.rows.row_off, g.rows.B, (int64_t)blockIdx.y * cut.rows);
+    if (b < 0) return;
     const Seq s = seq_of(g.rows, b, g.state != nullptr);
-    const int cells = g.heads * g.head_dim * g.state_dim, i = blockIdx.x * 256 + threadIdx.x;
-    if (s.count <= 0 || i >= cells) return;
-    const int h = i / (g.head_dim * g.state_dim), segs = min((s.count + cut.rows - 1) / cut.rows, cut.count);
-    float v = g.state && s.pos > 0 ? g.state[(size_t)s.slot * cells + i] : 0.0f;
-    float *at = cut.states + (size_t)b * cut.count * cells + i;
-    const float *decay = cut.decays + (size_t)b * cut.count * g.heads + h;
-    at[0] = v;
-    constexpr int AHEAD = 8;   // segments on their way from memory at once
-    for (int k = 1; k < segs; k += AHEAD) {
-        float own[AHEAD], d[AHEAD];
+    if (s.count <= cut.rows || (gridDim.y != (unsigned)g.rows.B && (s.row + cut.rows - 1) / cut.rows != (int64_t)blockIdx.y)) return;
+    const int cells = g.heads * g.head_dim * g.state_dim, slot0 = (int)s.row / (cut.rows / 2), segs = (int)(((int64_t)s.count + cut.rows - 1) / cut.rows);
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < cells; i += gridDim.x * 256) {
+        const int h = i / (g.head_dim * g.state_dim);
+        float v = g.state && s.pos > 0 ? g.state[(size_t)s.slot * cells + i] : 0.0f;
+        float *at = cut.states + (size_t)slot0 * cells + i;
+        const float *decay = cut.decays + (size_t)slot0 * g.heads + h;
+        at[0] = v;
+        constexpr int AHEAD = 8;   // segments on their way from memory at once
+        for (int k = 1; k < segs; k += AHEAD) {
+            float own[AHEAD], d[AHEAD];
 #pragma unroll
-        for (int e = 0; e < AHEAD; ++e) {
-            const int n = min(k + e, segs - 1);
-            own[e] = at[(size_t)n * cells], d[e] = decay[(size_t)(n - 1) * g.heads];
-        }
+            for (int e = 0; e < AHEAD; ++e) {
+                const int n = min(k + e, segs - 1);
+                own[e] = at[(size_t)n * cells], d[e] = decay[(size_t)(n - 1) * g.heads];
+            }
 #pragma unroll
-        for (int e = 0; e < AHEAD; ++e) {
-            if (k + e >= segs) break;
-            v = fmaf(__builtin_amdgcn_exp2f(d[e]), v, own[e]);
-            at[(size_t)(k + e) * cells] = v;
+            for (int e = 0; e < AHEAD; ++e) {
+                if (k + e >= segs) break;
+                v = fmaf(__builtin_amdgcn_exp2f(d[e]), v, own[e]);
+                at[(size_t)(k + e) * cells] = v;
+            }
         }
     }
 }
@@ -1108,7 +1121,7 @@ static void norm_by_width(const mdf_block_norm_args &a, hipStream_t st)
 
 // How a call's sequences are cut.  Unsplit there is a workgroup per sequence and four blocks of 32 channels.
 struct ScanPlan {
-    int unit_blocks, seg_rows, segs;
+    int unit_blocks, seg_rows, slots, items;
     size_t state_floats, decay_floats;
 };
 static ScanPlan scan_plan(const mdf_scan_args &a)
@@ -1116,33 +1129,36 @@ static ScanPlan scan_plan(const mdf_scan_args &a)
     ScanPlan p = {};
     const int pblocks = (a.head_dim + 31) / 32;
     p.unit_blocks = a.groups * ((a.heads / a.groups * pblocks + SCAN_WAVES - 1) / SCAN_WAVES);
-    p.segs = 1;
     // `even`: rows per workgroup if all were equally long, two per CU (512).  A sequence much longer than that is what a call waits for, and the calls it
     // holds up are cut although making the states first costs half as much again: 32 768 rows of 16 heads take 162 us in 64 segments (191 in 128, 182
-    // in 32, 580 in 8); 48 mixed lengths to 1 024 of 8 heads in float32 137 us in segments of 256, 150 uncut.  Under 256 rows the carried states outweigh it.
+    // in 32, 580 in 8); 48 mixed lengths to 1 024 of 8 heads in float32 127 us in segments of 256, 150 uncut.  Under 256 rows the carried states outweigh it.
+    // Beside 32 / 128 sequences of one row the 32 768 rows take 187 / 207 us, 3 000 where they are not cut.
     const int64_t even = a.rows.R * p.unit_blocks / 512;
     if (a.rows.max_len > 512 && (int64_t)a.rows.max_len * 2 > even * 5) {
-        const int rows = (int)std::max<int64_t>(256, (even + 63) / 64 * 64), segs = (a.rows.max_len + rows - 1) / rows;
-        const size_t cells = (size_t)a.heads * a.head_dim * a.state_dim;
-        if (segs > 1 && (size_t)a.rows.B * segs * cells <= (size_t)1 << 28) {   // (a workspace of 1 GiB)
+        const int rows = (int)std::max<int64_t>(256, (even + 63) / 64 * 64);
+        if (a.rows.max_len > rows) {
+            // some 1 024 / unit_blocks slots at most, since rows >= even: a workspace of 65 MiB whatever the lengths, for a workgroup's part of a state is 128 x 128
             p.seg_rows = rows;
-            p.segs = segs;
-            p.state_floats = (size_t)a.rows.B * segs * cells;
-            p.decay_floats = (size_t)a.rows.B * segs * a.heads;
+            p.slots = (int)(a.rows.R * 2 / rows);
+            p.state_floats = (size_t)p.slots * a.heads * a.head_dim * a.state_dim;
+            p.decay_floats = (size_t)p.slots * a.heads;
         }
     }
+    p.items = a.rows.B + p.slots;
     return p;
 }
 
 template <typename T, int NT, bool WORDS>
 static void scan_launch(const mdf_scan_args &a, const ScanPlan &p, void *workspace, hipStream_t st)
 {
-    ScanSplit cut = {p.seg_rows, p.segs, static_cast<float *>(workspace), static_cast<float *>(workspace) + p.state_floats};
-    const int items = a.rows.B * p.segs;
+    ScanSplit cut = {p.seg_rows, p.slots, static_cast<float *>(workspace), static_cast<float *>(workspace) + p.state_floats};
+    const int items = p.items;
     const dim3 grid((unsigned)((items + 7) / 8 * 8 * p.unit_blocks)), block(64 * SCAN_WAVES);
     if (p.seg_rows) {
         hipLaunchKernelGGL((k_scan<T, NT, true, WORDS>), grid, block, 0, st, a, cut, items, p.unit_blocks);
-        hipLaunchKernelGGL(k_scan_carry, dim3((unsigned)((a.heads * a.head_dim * a.state_dim + 255) / 256), (unsigned)a.rows.B), dim3(256), 0, st, a, cut);
+        // some 4 096 workgroups: most find no sequence where the few long ones are among many
+        const unsigned y = (unsigned)std::min<int64_t>(a.rows.B, a.rows.R / p.seg_rows + 1), x = (unsigned)((a.heads * a.head_dim * a.state_dim + 255) / 256);
+        hipLaunchKernelGGL(k_scan_carry, dim3(y == 1 ? x : std::min(x, std::max(4096 / y, 1u)), y), dim3(256), 0, st, a, cut);
     }
     hipLaunchKernelGGL((k_scan<T, NT, false, WORDS>), grid, block, 0, st, a, cut, items, p.unit_blocks);
 }
@@ -1283,7 +1299,7 @@ static int check_scan(const mdf_scan_args *a)
                     !overlap(a->c, a->ldc, gn, e, a->y, a->ldy, hp, e, R) && !overlap(a->dt, a->lddt, a->heads, dt_size(a->dt_dtype), a->y, a->ldy, hp, e, R),
                 "selective_scan_dev: y overlaps an input");
     const ScanPlan p = scan_plan(*a);
-    MDF_REQUIRE(((int64_t)a->rows.B * p.segs + 7) / 8 * 8 * p.unit_blocks < (int64_t)1 << 31 && (int64_t)a->heads * a->head_dim * a->state_dim < (int64_t)1 << 31 && a->rows.B <= 65535 * (p.seg_rows ? 1 : 32768),
+    MDF_REQUIRE(((int64_t)p.items + 7) / 8 * 8 * p.unit_blocks < (int64_t)1 << 31 && (int64_t)a->heads * a->head_dim * a->state_dim < (int64_t)1 << 31,
                 "selective_scan_dev: %d sequences of %d heads are too many for one call", a->rows.B, a->heads);
     return MDF_OK;
 }

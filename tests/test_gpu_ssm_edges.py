@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import ssm_oracle as orc
-from test_gpu_ssm import TYPES, f64, scan_inputs, ssm
+from test_gpu_ssm import TYPES, check_scan, f64, near, scan_inputs, ssm
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -70,3 +70,25 @@ def test_a_residual_scale_changed_in_place_is_the_one_used():
         assert bool((got == k).all())
     with pytest.raises(ValueError, match="host"):
         ssm().block_norm(s, residual=r, scale=scale.cuda())
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# long sequences among short ones
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[2600] + [1] * 40, [1] * 300 + [2100] + [0] * 5 + [1] * 200, [255, 256, 257, 0, 511, 512, 513, 768, 0, 0, 1025, 1, 256, 769], [1, 1400, 3, 1200, 0, 257, 2]])
+def test_scan_cuts_long_sequences_among_short_ones(dtype, lens):
+    """Lengths on both sides of whole segments, behind any number of short and empty sequences, with states that begin and continue."""
+    check_scan(*scan_inputs(221, lens, 2, 1, 32, 24, dtype, kept=True))
+
+
+def test_scan_cuts_a_long_sequence_among_more_sequences_than_a_grid_is_high():
+    rows, x, dt, a, b, c, kw = scan_inputs(222, [1] * 70000 + [1500], 1, 1, 32, 8, "f32")
+    got = ssm().selective_scan(x, dt, a, b, c, rows, **kw)
+    alone = ssm().SequenceRows.build([1500])
+    last = lambda t: t[70000:]  # noqa: E731
+    want, slack, _ = orc.scan(f64(last(x)), f64(last(dt)), f64(a), f64(last(b)), f64(last(c)), [1500], [0], d=f64(kw["d"]), dt_bias=f64(kw["dt_bias"]))
+    near(last(got), want, slack)
+    near(ssm().selective_scan(last(x), last(dt), a, last(b), last(c), alone, **kw), want, slack)
+    once = ssm().SequenceRows.build([1] * 70000)
+    assert torch.equal(got[:70000], ssm().selective_scan(x[:70000], dt[:70000], a, b[:70000], c[:70000], once, **kw))

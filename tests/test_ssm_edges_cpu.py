@@ -75,3 +75,44 @@ def test_a_scale_on_a_gpu_is_refused():
         ssm.block_norm(torch.zeros(3, 8), eps=OnGpu())
     with pytest.raises(ValueError, match="groups.*host"):
         ssm.block_norm(torch.zeros(3, 8), groups=OnGpu())
+
+
+def _scan_args(R, B, max_len, heads=16, groups=1, head_dim=64, state_dim=128):
+    from mDeepFRI import _hip
+    P, a = 1 << 40, ssm._Scan()                        # addresses that nothing reads
+    a.rows.lengths, a.rows.row_off, a.rows.R, a.rows.B, a.rows.max_len = P, P, R, B, max_len
+    a.x, a.b, a.c, a.dt, a.a, a.y = (k * P for k in range(1, 7))
+    a.ldx = a.ldy = heads * head_dim
+    a.ldb = a.ldc = groups * state_dim
+    a.lddt, a.heads, a.groups, a.head_dim, a.state_dim, a.dtype, a.dt_dtype = heads, heads, groups, head_dim, state_dim, _hip.DT_BF16, _hip.DT_BF16
+    return a
+
+
+@pytest.mark.parametrize("short", [0, 1, 32, 128, 5000, 70000])
+def test_a_long_prompt_beside_many_short_sequences_is_cut_all_the_same(short):
+    """The workspace goes by the rows, not by sequences times segments, and no number of sequences refuses the cut."""
+    import ctypes
+    from mDeepFRI import _hip
+    a = _scan_args(32768 + short, 1 + short, 32768)
+    need = _hip.lib().mdf_scan_workspace_bytes(ctypes.byref(a))
+    state = 16 * 64 * 128 * 4
+    assert 32 * state < need <= 65 << 20
+    if _hip.device_count() == 0:
+        assert _hip.lib().mdf_selective_scan_dev(ctypes.byref(a), 1 << 45, need, None) == _hip.MDF_ENODEVICE
+    assert _hip.lib().mdf_selective_scan_dev(ctypes.byref(a), 1 << 45, need - 1, None) == _hip.MDF_ECAPACITY
+
+
+def test_workspace_of_the_scan_is_bounded():
+    """Any sizes: at most 65 MiB, none where no sequence is long."""
+    import ctypes
+    import random
+    from mDeepFRI import _hip
+    rng = random.Random(7)
+    for _ in range(2000):
+        groups = rng.choice([1, 1, 2, 8])
+        R, heads = rng.choice([600, 5000, 40000, 10**6, 2**31 - 1]), groups * rng.choice([1, 2, 16, 128, 4096])
+        a = _scan_args(R, rng.choice([1, 7, 1000]), rng.choice([0, 512, 513, R // 3, R]), heads, groups, rng.choice([1, 32, 40, 64, 256]), rng.choice([1, 16, 128]))
+        if a.heads * a.head_dim >= 1 << 23:
+            continue
+        need = _hip.lib().mdf_scan_workspace_bytes(ctypes.byref(a))
+        assert need <= 65 << 20 and (need == 0 or a.rows.max_len > 512), (R, heads, a.rows.max_len)
