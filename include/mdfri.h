@@ -257,7 +257,7 @@ typedef struct {
 
 /* out[t][c] = act(bias[c] + sum_k weight[k][c] * x[t - (width-1) + k][c]) along every sequence, act = silu or none; inputs before the sequence's
  * first token are 0.  state (n_slots, width, channels), of x's type: the input of token t (counted over all calls) is kept at entry
- * t mod width.  out must not overlap x.  width 1..8. */
+ * t mod width.  out must not overlap x.  width 1..8; tiles of 8 rows times pieces of 16 bytes in a row: below 2^32. */
 typedef struct {
     mdf_seq_rows rows;
     const void *x;
@@ -275,7 +275,7 @@ int mdf_causal_conv_dev(const mdf_conv_args *args, void *stream);
  * over every sequence; H is f32, state (n_slots, heads, head_dim, state_dim).  x, y: (R, heads, head_dim), b, c: (R, groups, state_dim), each
  * contiguous inside a row, row strides at least a row's width; dt (R, heads) of any of the three types.  y must not overlap an input.  head_dim 1..256, state_dim 1..128.
  * Non-finite values stay where the recurrence puts them: nothing before the token or beside the channel they enter by is touched (an
- * infinity may come out as NaN). */
+ * infinity may come out as NaN).  Sequences (and 1 024 segments of long ones) times groups times a quarter of a group's blocks of 32 channels: below 2^31. */
 typedef struct {
     mdf_seq_rows rows;
     const void *x, *b, *c, *dt;

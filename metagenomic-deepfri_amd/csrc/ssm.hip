@@ -367,6 +367,7 @@ template <> struct Terms<F16> { static constexpr int X = 2, IN = 2; };
 template <> struct Terms<float> { static constexpr int X = 3, IN = 2; };
 
 constexpr int SCAN_Q = 32, SCAN_WAVES = 4;
+constexpr unsigned GRID_X = 1u << 23;   // most workgroups of 256 threads in a launch's x: a dimension of a grid holds fewer than 2^32 threads
 
 // A value the compiler may not compute with ahead of here: what is derived from it in a loop (offsets, comparisons) is made where it is used, one instruction
 // each, instead of being kept in dozens of registers over the loop
@@ -423,7 +424,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
     __shared__ __align__(16) T Xs[SCAN_WAVES][SCAN_Q][PS];
     __shared__ __align__(16) float steps[SCAN_WAVES][2][6][SCAN_Q];   // k = c - log2 D, c, low part of k, D 2^(c_31 - c), 2^c, low part of c, of two chunks
     // Block -> (item, channels): workgroups of one item (which read the same B and C) lie on one XCD -- block b runs on XCD b mod 8 -- and close in time.
-    const int xcd = blockIdx.x & 7, place = blockIdx.x >> 3, item = (place / unit_blocks) * 8 + xcd, ub = place % unit_blocks;
+    const int xcd = blockIdx.x & 7, place = (int)(blockIdx.y * (GRID_X / 8) + (blockIdx.x >> 3)), item = (place / unit_blocks) * 8 + xcd, ub = place % unit_blocks;
     if (item >= items) return;
     // items: the slots of segments, then the sequences that are not cut
     const int b = item >= cut.slots ? item - cut.slots : __builtin_amdgcn_readfirstlane(slot_owner(g.rows, cut, item));
@@ -1153,7 +1154,8 @@ static void scan_launch(const mdf_scan_args &a, const ScanPlan &p, void *workspa
 {
     ScanSplit cut = {p.seg_rows, p.slots, static_cast<float *>(workspace), static_cast<float *>(workspace) + p.state_floats};
     const int items = p.items;
-    const dim3 grid((unsigned)((items + 7) / 8 * 8 * p.unit_blocks)), block(64 * SCAN_WAVES);
+    const unsigned blocks = (unsigned)((items + 7) / 8 * 8) * p.unit_blocks;
+    const dim3 grid(std::min(blocks, GRID_X), (blocks + GRID_X - 1) / GRID_X), block(64 * SCAN_WAVES);
     if (p.seg_rows) {
         hipLaunchKernelGGL((k_scan<T, NT, true, WORDS>), grid, block, 0, st, a, cut, items, p.unit_blocks);
         // some 4 096 workgroups: most find no sequence where the few long ones are among many
@@ -1253,8 +1255,6 @@ int mdf_causal_conv_dev(const mdf_conv_args *a, void *stream)
     MDF_REQUIRE(a->ldx >= 0 && (a->ldo >= a->channels || a->rows.R == 1), "causal_conv_dev: row strides %lld, %lld for %d channels", (long long)a->ldx, (long long)a->ldo, a->channels);
     const size_t e = dt_size(a->dtype);
     MDF_REQUIRE(!overlap(a->x, a->ldx, a->channels, e, a->out, a->ldo, a->channels, e, a->rows.R), "causal_conv_dev: out overlaps x");
-    if (int rc = require_device()) return rc;
-    hipStream_t st = static_cast<hipStream_t>(stream);
     const int v = a->channels >= 16 / (int)e ? 16 / (int)e : 1;
     const int lanes = (a->channels + v - 1) / v;
     // Tiles per thread: further ones save the weights, the rows in front and a search, and cost parallel threads; they pay once one tile each is more than
@@ -1267,7 +1267,9 @@ int mdf_causal_conv_dev(const mdf_conv_args *a, void *stream)
     if (e == 4) steps = units >= 6 ? 4 : 1;
     else if (a->width > 2 && units >= 3) steps = a->width > 4 && units >= 5 ? 4 : 2;
     const int64_t threads = (tiles + steps - 1) / steps * lanes;
-    MDF_REQUIRE((threads + 255) / 256 < (int64_t)1 << 31, "causal_conv_dev: %lld rows of %d channels are too many", (long long)a->rows.R, a->channels);
+    MDF_REQUIRE((threads + 255) / 256 < 2 * (int64_t)GRID_X, "causal_conv_dev: %lld rows of %d channels are too many", (long long)a->rows.R, a->channels);
+    if (int rc = require_device()) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)((threads + 255) / 256));
     MDF_BY_TYPE(a->dtype, T, {
         if (v > 1) conv_launch<T, 16 / sizeof(T)>(*a, steps, lanes, grid, st);
@@ -1347,7 +1349,21 @@ int mdf_selective_step_dev(const mdf_step_args *a, void *stream)
                 "selective_step_dev: y overlaps an input");
     if (int rc = require_device()) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    MDF_BY_TYPE(a->dtype, T, step_launch<T>(*a, st));
+    mdf_step_args k = *a;
+    for (int64_t b = 0; b < a->B; b += GRID_X) {   // a workgroup at least per sequence, in x
+        k.B = (int32_t)std::min<int64_t>(GRID_X, a->B - b);
+        k.xbc = static_cast<const char *>(a->xbc) + (size_t)b * a->ldx * e;
+        k.dt = static_cast<const char *>(a->dt) + (size_t)b * a->lddt * dt_size(a->dt_dtype);
+        k.y = static_cast<char *>(a->y) + (size_t)b * a->ldy * e;
+        if (a->positions) k.positions = a->positions + b;
+        if (a->slots) k.slots = a->slots + b;
+        else {
+            k.n_slots = a->n_slots - (int32_t)b;
+            k.conv_state = static_cast<char *>(a->conv_state) + (size_t)b * a->width * ch * e;
+            k.state = a->state + (size_t)b * hp * a->state_dim;
+        }
+        MDF_BY_TYPE(a->dtype, T, step_launch<T>(k, st));
+    }
     MDF_HIP(hipGetLastError());
     return MDF_OK;
 }
@@ -1382,11 +1398,17 @@ int mdf_block_norm_dev(const mdf_block_norm_args *a, void *stream)
     if (int rc = require_device()) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     mdf_block_norm_args k = *a;
-    if (!has_out) k.out = nullptr;
-    MDF_BY_TYPE(a->dtype, T, {
-        if (a->residual && a->residual_dtype == MDF_DT_F32) norm_by_width<T, float>(k, st);
-        else norm_by_width<T, T>(k, st);
-    });
+    constexpr int64_t ROWS = 1 << 21;   // of one launch: up to 1 024 threads each in x
+    for (int64_t r = 0; r < a->rows; r += ROWS) {
+        auto at = [&](auto *p, int64_t ld, size_t size) { return p ? (decltype(p))((uintptr_t)p + (size_t)r * ld * size) : p; };
+        k.rows = std::min(ROWS, a->rows - r);
+        k.s = at(a->s, a->lds, e), k.gate = at(a->gate, a->ldg, e), k.residual = at(a->residual, a->ldr, er);
+        k.residual_out = at(a->residual_out, a->ldro, er), k.out = has_out ? at(a->out, a->ldo, e) : nullptr;
+        MDF_BY_TYPE(a->dtype, T, {
+            if (a->residual && a->residual_dtype == MDF_DT_F32) norm_by_width<T, float>(k, st);
+            else norm_by_width<T, T>(k, st);
+        });
+    }
     MDF_HIP(hipGetLastError());
     return MDF_OK;
 }

@@ -92,3 +92,88 @@ def test_scan_cuts_a_long_sequence_among_more_sequences_than_a_grid_is_high():
     near(ssm().selective_scan(last(x), last(dt), a, last(b), last(c), alone, **kw), want, slack)
     once = ssm().SequenceRows.build([1] * 70000)
     assert torch.equal(got[:70000], ssm().selective_scan(x[:70000], dt[:70000], a, b[:70000], c[:70000], once, **kw))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# more rows than one dimension of a grid holds
+# ---------------------------------------------------------------------------------------------------------------------
+def same_rows(got, make, rows, step=1 << 24):
+    """`got` against make(slice) piece by piece (a whole float64 copy would be large)."""
+    for r in range(0, rows, step):
+        at = slice(r, min(r + step, rows))
+        want, slack = make(at)
+        assert bool(((got[at].double() - want).abs() <= slack).all()), r
+
+
+def test_norm_of_2_to_26_rows():
+    """Per-head norms of a long batch: 64 threads a row pass 2^32 threads."""
+    rows, dim = 2**26 + 5, 4
+    g = torch.Generator(device="cuda").manual_seed(231)
+    s = torch.randn(rows, dim, generator=g, device="cuda")
+    w = torch.tensor([1.0, 2.0, 0.5, -1.0], device="cuda")
+    _, got = ssm().block_norm(s, post_weight=w, eps=1e-6)
+
+    def make(at):
+        v = s[at].double()
+        want = v / torch.sqrt((v * v).mean(1, keepdim=True) + 1e-6) * w.double()
+        return want, want.abs() * 16 * 2.0**-24 + 1e-36      # a sum of 4 squares, a mean, a root, a division and two products
+    same_rows(got, make, rows)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norm_of_rows_in_several_launches_in_place(dtype):
+    """Gate, residual and both outputs in place over 2^21 + 3 rows: each row as by itself."""
+    rows, dim = 2**21 + 3, 24
+    g = torch.Generator(device="cuda").manual_seed(232)
+    s, gate = (torch.randn(rows, dim + 8, generator=g, device="cuda").to(TYPES[dtype])[:, 8:] for _ in range(2))
+    res = torch.randn(rows, dim, generator=g, device="cuda")
+    kw = dict(post_weight=torch.rand(dim, generator=g, device="cuda"), pre_weight=torch.rand(dim, generator=g, device="cuda"), scale=0.5)
+    some = [0, 1, 2**21 - 1, 2**21, 2**21 + 1, 2**21 + 2]
+    want_r, want = ssm().block_norm(s[some], gate=gate[some], residual=res[some], **kw)
+    half = ssm().block_norm(s[2**20:], gate=gate[2**20:], residual=res[2**20:], **kw)
+    r, out = ssm().block_norm(s, gate=gate, residual=res, residual_out=res, out=s, **kw)
+    assert torch.equal(r[some], want_r) and torch.equal(out[some], want)
+    assert torch.equal(r[2**20:], half[0]) and torch.equal(out[2**20:], half[1])
+
+
+def test_scan_of_2_to_24_sequences():
+    """One-row sequences, a workgroup each: y = (c b D + d) x."""
+    n = 2**24 + 9
+    g = torch.Generator(device="cuda").manual_seed(233)
+    x, b, c = (torch.randn(n, 1, 1, generator=g, device="cuda") for _ in range(3))
+    dt, a = torch.randn(n, 1, generator=g, device="cuda"), torch.tensor([-1.0], device="cuda")
+    lengths, off = torch.ones(n, dtype=torch.int32, device="cuda"), torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    got = ssm().selective_scan(x, dt, a, b, c, ssm().SequenceRows(lengths, off, 1, dense=True))
+
+    def make(at):
+        want = c[at].double() * b[at].double() * torch.nn.functional.softplus(dt[at].double(), threshold=100).unsqueeze(2) * x[at].double()
+        return want, want.abs() * 40 * 2.0**-24 + 1e-36      # softplus 12 + |dt| steps and the products' dropped terms
+    same_rows(got, make, n)
+
+
+def test_step_of_2_to_24_sequences():
+    """Width 1 without a bias: u = silu(w xbc), y = u_c u_b D u_x, in their own states and in chosen ones."""
+    n = 2**24 + 3
+    g = torch.Generator(device="cuda").manual_seed(234)
+    xbc, dt = torch.randn(n, 3, generator=g, device="cuda"), torch.randn(n, 1, generator=g, device="cuda")
+    w, a = torch.tensor([[1.0, -2.0, 0.5]], device="cuda"), torch.tensor([-1.0], device="cuda")
+    ring, state = torch.full((n, 1, 3), 7.0, device="cuda"), torch.full((n, 1, 1, 1), 7.0, device="cuda")
+    got = ssm().selective_step(xbc, dt, a, conv_weight=w, conv_state=ring, state=state).clone()
+
+    def parts(at):
+        u = w.double() * xbc[at].double()
+        u = u * torch.sigmoid(u)
+        h = torch.nn.functional.softplus(dt[at].double(), threshold=100) * u[:, :1] * u[:, 1:2]
+        return u, h
+
+    def make(at):
+        u, h = parts(at)
+        want = (h * u[:, 2:]).unsqueeze(2)
+        return want, want.abs() * 100 * 2.0**-24 + 1e-36     # three silu of 8 + 2 |u| steps, |u| < 12, a softplus of 12 + |dt|, three products
+    same_rows(got, make, n)
+    same_rows(state, lambda at: (parts(at)[1].view(-1, 1, 1, 1), parts(at)[1].abs().view(-1, 1, 1, 1) * 80 * 2.0**-24 + 1e-36), n)
+    assert torch.equal(ring[:, 0], xbc)
+    slots = torch.arange(n - 1, -1, -1, dtype=torch.int32, device="cuda")
+    again, ring2, state2 = ssm().selective_step, torch.zeros_like(ring), torch.zeros_like(state)
+    assert torch.equal(again(xbc, dt, a, conv_weight=w, conv_state=ring2, state=state2, slots=slots), got)
+    assert torch.equal(state2.flip(0), state) and torch.equal(ring2.flip(0), ring)

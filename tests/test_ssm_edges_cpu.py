@@ -116,3 +116,29 @@ def test_workspace_of_the_scan_is_bounded():
             continue
         need = _hip.lib().mdf_scan_workspace_bytes(ctypes.byref(a))
         assert need <= 65 << 20 and (need == 0 or a.rows.max_len > 512), (R, heads, a.rows.max_len)
+
+
+@pytest.mark.parametrize("channels, fits", [(8 * 127, True), (8 * 127 + 1, False)])
+def test_a_convolution_larger_than_a_grid_is_refused(channels, fits):
+    """A dimension of a grid holds fewer than 2^32 threads: 2^28 rows are 2^25 tiles, of 128 lanes for 1 017 and more bfloat16 channels."""
+    from mDeepFRI import _hip
+    a = ssm._Conv()
+    a.rows.lengths, a.rows.row_off, a.rows.R, a.rows.B, a.rows.max_len = 1 << 40, 1 << 40, 1 << 28, 1, 1 << 28
+    a.x, a.weight, a.out, a.ldx, a.ldo, a.channels, a.width, a.dtype = 1 << 41, 1 << 40, 1 << 45, channels, channels, channels, 2, _hip.DT_BF16
+    if fits and _hip.device_count() > 0:
+        pytest.skip("a GPU is visible")
+    import ctypes
+    rc = _hip.lib().mdf_causal_conv_dev(ctypes.byref(a), None)
+    assert rc == (_hip.MDF_ENODEVICE if fits else _hip.MDF_EINVAL) and (fits or "too many" in _hip.last_error())
+
+
+@pytest.mark.parametrize("sequences, fits", [(2**23 - 1, True), (2**28 - 8, True), (2**28, False)])
+def test_a_scan_of_more_workgroups_than_the_library_counts_is_refused(sequences, fits):
+    """2^31 workgroups: 8 per sequence here; every smaller number takes as many rows of the grid as it needs."""
+    import ctypes
+    from mDeepFRI import _hip
+    a = _scan_args(2**31 - 1, sequences, 1)
+    if fits and _hip.device_count() > 0:
+        pytest.skip("a GPU is visible")
+    rc = _hip.lib().mdf_selective_scan_dev(ctypes.byref(a), None, 0, None)
+    assert rc == (_hip.MDF_ENODEVICE if fits else _hip.MDF_EINVAL) and (fits or "too many" in _hip.last_error())
