@@ -2639,9 +2639,16 @@ int mdf_lm_forward_dev(mdf_lm *lm, const uint8_t *seq_idx, const int64_t *prot_r
                 unsigned *async_ = lm->sync;
                 void *args[] = {&aU1, &aW2, &aU2, &atab, &ab2, &alet, &len_dev, &aB, &aL, &ah1, &ah2, &prot_row, &h_out, &async_};
                 const hipError_t le = hipLaunchCooperativeKernel(fn, dim3(H / 2), dim3(256), args, 0, st);
-                if (le != hipSuccess) {   // refused, nothing launched: too large a grid, or (hipErrorIllegalState) another process holds the device's cooperative queue
-                    (void)hipGetLastError();
+                // Refused, nothing launched: too large a grid for what is free, or (hipErrorIllegalState) another process holds the device's cooperative queue.
+                // Any other error is no refusal (a kernel image that does not load, the failure of earlier work) and is the caller's to see.
+                if (le == hipErrorCooperativeLaunchTooLarge || le == hipErrorLaunchOutOfResources || le == hipErrorIllegalState) {
+                    (void)hipGetLastError();   // left behind it would fail the next launch
                     fits = false;
+                    static bool warned = false;
+                    if (!warned) fprintf(stderr, "libmdfri_hip: persistent LSTM launch refused (%s); using the per-step GEMM form\n", hipGetErrorName(le));
+                    warned = true;
+                } else {
+                    MDF_HIP(le);
                 }
             }
         }
