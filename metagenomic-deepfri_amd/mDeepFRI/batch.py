@@ -23,13 +23,14 @@ from . import _hip
 # that has not read them yet -- tests/conftest.py, pytest_collection_finish), which a process that builds a Predictor first would pay.
 try:
     import torch as _torch_module
-except ImportError:          # host-side packing and planning need no torch
-    _torch_module = None
+    _torch_error = None
+except (ImportError, OSError) as e:          # none, or one whose libraries do not load; host-side packing and planning need no torch
+    _torch_module, _torch_error = None, e
 
 
 def _torch():
     if _torch_module is None:
-        raise ImportError("mDeepFRI.batch needs PyTorch-ROCm for device memory and streams")
+        raise ImportError(f"mDeepFRI.batch needs PyTorch-ROCm for device memory and streams: {_torch_error}") from _torch_error
     return _torch_module
 
 
