@@ -8,7 +8,7 @@
 They stand beside the recurrent and convolutional sequence models of this package (mDeepFRI.predict: LSTM branch, CNN) for features of a block
     x -> pre-norm -> in-projection -> causal_conv -> selective_scan -> block_norm(gate=z, gate_first=True) -> out-projection -> block_norm(residual=...)
 whose two projections are products of the caller's.  The reference has nothing of the kind; inference only: a tensor that asks for a gradient
-is refused.
+or carries a tangent is refused.
 
 Tensors are torch tensors on one GPU; work is enqueued on that GPU's current stream and nothing waits for it.  Rows of no sequence and
 of a skipped one are left as they were in an `out` that is handed in and are zero in one that is made here.  Outputs are f32, bfloat16 or float16 like their
@@ -211,6 +211,18 @@ def _grad() -> bool:
     return _torch().is_grad_enabled()
 
 
+def _dual_level() -> bool:
+    """Whether forward-mode derivatives are being taken (a private name: without it the tensors are asked at every call)."""
+    return getattr(_torch().autograd.forward_ad, "_current_level", 0) >= 0
+
+
+def _refuse_tangents(**tensors) -> None:
+    """Forward-mode derivatives, which requires_grad does not show.  At every call: a tangent is no part of a tensor's form."""
+    for name, t in tensors.items():
+        if t is not None and _torch().autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} carries a tangent: the state-space operators are inference only")
+
+
 def _made(out, like, rows: SequenceRows, shape):
     """(`zero_skipped` is set for an output made here, so one whose every row is a sequence's needs no zeros)"""
     if out is not None:
@@ -247,6 +259,8 @@ def causal_conv(x, weight, rows: SequenceRows, *, bias=None, silu: bool = True, 
     x (R, channels), any row stride; weight (width, channels) and bias (channels) f32, width 1..8; silu: the activation, or none.  state
     (n_slots, width, channels) of x's type keeps the last inputs (token t at entry t mod width) from call to call: `slots` (B) says which one
     each sequence owns (default: its own number), `positions` (B) how many tokens it had before (default 0: a new sequence)."""
+    if _dual_level():
+        _refuse_tangents(x=x, weight=weight, bias=bias, state=state, out=out)
     device = x.device
 
     def check():
@@ -277,6 +291,8 @@ def selective_scan(x, dt, a, b, c, rows: SequenceRows, *, d=None, dt_bias=None, 
     row strides are free; a, d, dt_bias (heads) f32.  head_dim 1..256, state_dim 1..128, heads a multiple of groups.  state (n_slots, heads,
     head_dim, state_dim) f32 is continued where positions > 0 and left behind for the next call; slots / positions as in causal_conv.
     dt = -infinity masks a token: the state passes it unchanged (y still holds H c + d x)."""
+    if _dual_level():
+        _refuse_tangents(x=x, dt=dt, a=a, b=b, c=c, d=d, dt_bias=dt_bias, state=state, out=out)
     device = x.device
 
     def check():
@@ -315,6 +331,8 @@ def selective_step(xbc, dt, a, *, conv_weight, conv_state, state, positions=None
     """One token of each of B sequences: causal_conv (silu) of xbc = [x | b | c] (B, heads*head_dim + 2*groups*state_dim), then selective_scan,
     in one launch; conv_state (n_slots, width, channels) and state (n_slots, heads, head_dim, state_dim) are updated in place.  Returns y
     (B, heads, head_dim).  The caller adds 1 to the positions of the sequences it continues."""
+    if _dual_level():
+        _refuse_tangents(xbc=xbc, dt=dt, a=a, conv_weight=conv_weight, conv_state=conv_state, state=state, conv_bias=conv_bias, d=d, dt_bias=dt_bias, out=out)
     device = xbc.device
 
     def check():
@@ -362,6 +380,8 @@ def block_norm(s, *, residual=None, gate=None, gate_act: str = "silu", gate_firs
     Returns (r or None, out or None); without a residual out is v, or pre(v).  post / pre: x / sqrt(mean(x^2) + eps) * weight + bias, of x less its
     mean with `center`; post on each of `groups` equal parts of a row.  scale, eps and groups are numbers on the host.  s and gate share a type; the residual
     is float32 or of that type, and r has its type.  residual_out may be the residual itself, out may be s or the gate."""
+    if _dual_level():
+        _refuse_tangents(s=s, residual=residual, gate=gate, post_weight=post_weight, post_bias=post_bias, scale_vec=scale_vec, pre_weight=pre_weight, pre_bias=pre_bias, residual_out=residual_out, out=out)
     device = s.device
     has_out = pre_weight is not None or residual is None
     scale, eps, groups = _number(scale, "scale"), _number(eps, "eps"), _number(groups, "groups", operator.index)

@@ -177,3 +177,15 @@ def test_step_of_2_to_24_sequences():
     again, ring2, state2 = ssm().selective_step, torch.zeros_like(ring), torch.zeros_like(state)
     assert torch.equal(again(xbc, dt, a, conv_weight=w, conv_state=ring2, state=state2, slots=slots), got)
     assert torch.equal(state2.flip(0), state) and torch.equal(ring2.flip(0), ring)
+
+
+def test_a_tangent_is_refused_in_a_call_of_a_known_form():
+    """What is kept of an earlier call's checks must not let it through."""
+    from torch.autograd import forward_ad
+    rows, x, dt, a, b, c, kw = scan_inputs(241, [9, 4], 2, 1, 32, 16, "f32")
+    want = ssm().selective_scan(x, dt, a, b, c, rows, **kw)
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="dt carries a tangent"):
+            ssm().selective_scan(x, forward_ad.make_dual(dt, torch.ones_like(dt)), a, b, c, rows, **kw)
+        assert torch.equal(ssm().selective_scan(x, dt, a, b, c, rows, **kw), want)
+    assert torch.equal(ssm().selective_scan(x, dt, a, b, c, rows, **kw), want)

@@ -142,3 +142,37 @@ def test_a_scan_of_more_workgroups_than_the_library_counts_is_refused(sequences,
         pytest.skip("a GPU is visible")
     rc = _hip.lib().mdf_selective_scan_dev(ctypes.byref(a), None, 0, None)
     assert rc == (_hip.MDF_ENODEVICE if fits else _hip.MDF_EINVAL) and (fits or "too many" in _hip.last_error())
+
+
+def _calls():
+    """Every operator with small arguments of the right forms: name -> (function, positional, keyword)."""
+    import torch
+    rows = ssm.SequenceRows.build([3, 2], device="cpu")
+    z, h = torch.zeros, dict(d=torch.zeros(2), dt_bias=torch.zeros(2))
+    return {
+        "causal_conv": (ssm.causal_conv, dict(x=z(5, 8), weight=z(4, 8), rows=rows), dict(bias=z(8), state=z(2, 4, 8), out=z(5, 8))),
+        "selective_scan": (ssm.selective_scan, dict(x=z(5, 2, 4), dt=z(5, 2), a=z(2), b=z(5, 1, 3), c=z(5, 1, 3), rows=rows), dict(h, state=z(2, 2, 4, 3), out=z(5, 2, 4))),
+        "selective_step": (ssm.selective_step, dict(xbc=z(2, 14), dt=z(2, 2), a=z(2)), dict(h, conv_weight=z(4, 14), conv_bias=z(14), conv_state=z(2, 4, 14), state=z(2, 2, 4, 3), out=z(2, 2, 4))),
+        "block_norm": (ssm.block_norm, dict(s=z(5, 8)), dict(residual=z(5, 8), gate=z(5, 8), post_weight=z(8), post_bias=z(8), scale_vec=z(8), pre_weight=z(8), pre_bias=z(8), residual_out=z(5, 8),
+                                                           out=z(5, 8))),
+    }
+
+
+@pytest.mark.parametrize("op", ["causal_conv", "selective_scan", "selective_step", "block_norm"])
+def test_every_tensor_with_a_tangent_is_refused(op):
+    """A forward-mode derivative would be lost without a word; also under no_grad, which does not stop forward mode."""
+    import torch
+    from torch.autograd import forward_ad
+    fn, args, more = _calls()[op]
+    args = {**args, **more}
+    with forward_ad.dual_level():
+        for name, t in args.items():
+            if not torch.is_tensor(t):
+                continue
+            dual = forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(ValueError, match=name + " carries a tangent"):
+                fn(**{**args, name: dual})
+            with torch.no_grad(), pytest.raises(ValueError, match=name + " carries a tangent"):
+                fn(**{**args, name: dual})
+        with pytest.raises(ValueError, match="not on a GPU"):        # none of them: the next check
+            fn(**args)
