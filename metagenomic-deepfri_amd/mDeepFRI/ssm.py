@@ -75,9 +75,11 @@ def _dtype(t, name: str) -> int:
 class SequenceRows:
     """Which rows belong to which sequence: `lengths` (B) and `row_off` (B+1), int32 device tensors, row_off ascending, and the longest length.
     `dense`: the caller's word that the sequences leave out no row of the first `total` (None: of any array that they are used with), whose outputs then need no
-    zeros when they are made here.  `build` makes one from host lengths, checks them and knows both."""
+    zeros when they are made here.  `build` makes one from host lengths, checks them and knows both.  The values in the tensors may change from call to call, and max_len
+    with them; another number of sequences is another SequenceRows."""
 
-    __slots__ = ("lengths", "row_off", "max_len", "dense", "total", "count", "form")
+    __slots__ = ("_lengths", "_row_off", "max_len", "dense", "total", "_count", "_form")
+    lengths, row_off, count, form = (property(operator.attrgetter("_" + name)) for name in ("lengths", "row_off", "count", "form"))   # not to be set: they were checked together
 
     def __init__(self, lengths, row_off, max_len: int, dense: bool = False, total: int | None = None):
         torch = _torch()
@@ -87,8 +89,8 @@ class SequenceRows:
             raise ValueError(f"row_off has {row_off.shape[0]} entries for {lengths.shape[0]} sequences (one more is wanted)")
         if lengths.device != row_off.device or max_len < 0:
             raise ValueError("lengths and row_off lie on different devices, or max_len is negative")
-        self.lengths, self.row_off, self.max_len, self.dense, self.total, self.count = lengths, row_off, int(max_len), dense, total, lengths.shape[0]
-        self.form = (self.count, lengths.get_device())
+        self._lengths, self._row_off, self.max_len, self.dense, self.total, self._count = lengths, row_off, int(max_len), dense, total, lengths.shape[0]
+        self._form = (self._count, lengths.get_device())
 
     @classmethod
     def build(cls, lengths, device="cuda", align: int = 1):

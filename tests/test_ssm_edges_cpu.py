@@ -176,3 +176,15 @@ def test_every_tensor_with_a_tangent_is_refused(op):
                 fn(**{**args, name: dual})
         with pytest.raises(ValueError, match="not on a GPU"):        # none of them: the next check
             fn(**args)
+
+
+def test_checked_tensors_of_rows_cannot_be_exchanged():
+    """The kernels go by the number of sequences that was checked: shorter tensors put in its place would be read past their ends."""
+    import torch
+    rows = ssm.SequenceRows.build([3, 0, 5], device="cpu")
+    for name in ("lengths", "row_off", "count", "form"):
+        with pytest.raises(AttributeError):
+            setattr(rows, name, torch.zeros(1, dtype=torch.int32))
+    assert rows.lengths.tolist() == [3, 0, 5] and rows.row_off.tolist() == [0, 3, 3, 8] and rows.count == 3 and rows.form == (3, -1)
+    rows.max_len = 7                                  # another batch of three in the same tensors
+    assert rows.max_len == 7
