@@ -239,7 +239,8 @@ int mdf_cnn_forward_dev(mdf_cnn *m, const uint8_t *seq_idx, const int32_t *Lq, c
  *
  * Sequence b owns rows [row_off[b], row_off[b] + lengths[b]) of R; row_off is ascending (mdf_layout_rows builds one; dense packing is as good)
  * and a length may be 0.  Rows of no sequence are neither read nor written.  `max_len` is the longest sequence (it sizes the split of long
- * sequences over workgroups, not the result: a longer one is still run to its end).
+ * sequences over workgroups; a longer one is still run to its end).  Whether the scan cuts a sequence, and where, goes by R and max_len of the call: the same
+ * sequence in another batch has the same results up to the order of float32 sums, not bit by bit.  The other operators' results do not depend on the batch.
  * Kept states: `slots[b]` (NULL: b) says which of the n_slots states sequence b continues and leaves behind, `positions[b]` (NULL: 0) how many tokens
  * it had before this call; at position 0 the old state is not read.  A sequence whose slot lies outside [0, n_slots) is skipped: its rows and
  * every state stay as they are (a padded batch).  The slots of one call must differ; the caller counts the positions.
@@ -274,8 +275,9 @@ int mdf_causal_conv_dev(const mdf_conv_args *args, void *stream);
  *     H[p][n] <- exp(D a[h]) H[p][n] + D x[t][h][p] b[t][g][n],     y[t][h][p] = sum_n H[p][n] c[t][g][n] + d[h] x[t][h][p]
  * over every sequence; H is f32, state (n_slots, heads, head_dim, state_dim).  x, y: (R, heads, head_dim), b, c: (R, groups, state_dim), each
  * contiguous inside a row, row strides at least a row's width; dt (R, heads) of any of the three types.  y must not overlap an input.  head_dim 1..256, state_dim 1..128.
- * Non-finite values stay where the recurrence puts them: nothing before the token or beside the channel they enter by is touched (an
- * infinity may come out as NaN).  Sequences (and 1 024 segments of long ones) times groups times a quarter of a group's blocks of 32 channels: below 2^31. */
+ * dt of -infinity (D = 0) passes the state on unchanged if the token's x and b are finite.  Non-finite values stay where the recurrence puts them: nothing before
+ * the token or beside the channel they enter by is touched (an infinity may come out as NaN).  Two tokens' b . c is formed in front of decays and step sizes: where
+ * it leaves float32's range, y does, however small these would make it.  Sequences (and 1 024 segments of long ones) times groups times a quarter of a group's blocks of 32 channels: below 2^31. */
 typedef struct {
     mdf_seq_rows rows;
     const void *x, *b, *c, *dt;

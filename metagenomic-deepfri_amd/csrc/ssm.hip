@@ -566,9 +566,10 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
         c += dpp_f64<0x118>(c);
         c += dpp_f64<0x142, 0xa>(c);     // ... and from lane 15 of the row below, into rows 1 and 3
         const double c31 = half ? lane_f64(c, 63) : lane_f64(c, 31);
-        // D_j 2^(c_i - c_j) = 2^(c_i - k_j), k = c - log2 D; D = 0 gives k = infinity and a factor of 0.  The logarithm as v_log and what it is off by.
+        // D_j 2^(c_i - c_j) = 2^(c_i - k_j), k = c - log2 D; D = 0 gives k = infinity and a factor of 0.  The logarithm as v_log and what it is off by; v_log takes a
+        // subnormal D for 0, and then 2^-lg is an infinity, which must not meet the one in lg.
         const float lg = __builtin_amdgcn_logf(D);
-        const float off = D > 0.0f ? fmaf(D, __builtin_amdgcn_exp2f(-lg), -1.0f) * 1.44269504f : 0.0f;
+        const float off = D >= 1.17549435e-38f ? fmaf(D, __builtin_amdgcn_exp2f(-lg), -1.0f) * 1.44269504f : 0.0f;
         const double kd = c - (double)lg - (double)off;
         const float hi = (float)c, khi = (float)kd;
         steps[wave][half][0][l32] = khi;

@@ -75,8 +75,8 @@ def _dtype(t, name: str) -> int:
 class SequenceRows:
     """Which rows belong to which sequence: `lengths` (B) and `row_off` (B+1), int32 device tensors, row_off ascending, and the longest length.
     `dense`: the caller's word that the sequences leave out no row of the first `total` (None: of any array that they are used with), whose outputs then need no
-    zeros when they are made here.  `build` makes one from host lengths, checks them and knows both.  The values in the tensors may change from call to call, and max_len
-    with them; another number of sequences is another SequenceRows."""
+    zeros when they are made here.  `build` makes one from host lengths, checks them and knows both.  The values in the tensors may change from call to call, max_len and
+    `dense` with them (a graph that is replayed with other lengths wants dense=False); another number of sequences is another SequenceRows."""
 
     __slots__ = ("_lengths", "_row_off", "max_len", "dense", "total", "_count", "_form")
     lengths, row_off, count, form = (property(operator.attrgetter("_" + name)) for name in ("lengths", "row_off", "count", "form"))   # not to be set: they were checked together
@@ -292,7 +292,8 @@ def selective_scan(x, dt, a, b, c, rows: SequenceRows, *, d=None, dt_bias=None, 
     x and the result (R, heads, head_dim), dt (R, heads), b and c (R, groups, state_dim) -- views into one wider array are fine, only the
     row strides are free; a, d, dt_bias (heads) f32.  head_dim 1..256, state_dim 1..128, heads a multiple of groups.  state (n_slots, heads,
     head_dim, state_dim) f32 is continued where positions > 0 and left behind for the next call; slots / positions as in causal_conv.
-    dt = -infinity masks a token: the state passes it unchanged (y still holds H c + d x)."""
+    dt = -infinity masks a token whose x and b are finite: the state passes it unchanged (y still holds H c + d x).  Long sequences may be cut and summed
+    in another order in another batch: the same to float32 rounding."""
     if _dual_level():
         _refuse_tangents(x=x, dt=dt, a=a, b=b, c=c, d=d, dt_bias=dt_bias, state=state, out=out)
     device = x.device

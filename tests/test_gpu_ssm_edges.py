@@ -189,3 +189,31 @@ def test_a_tangent_is_refused_in_a_call_of_a_known_form():
             ssm().selective_scan(x, forward_ad.make_dual(dt, torch.ones_like(dt)), a, b, c, rows, **kw)
         assert torch.equal(ssm().selective_scan(x, dt, a, b, c, rows, **kw), want)
     assert torch.equal(ssm().selective_scan(x, dt, a, b, c, rows, **kw), want)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# values at the ends of the range
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_scan_with_step_sizes_around_the_smallest_float32(dtype):
+    """softplus of -80 to -110: normal, subnormal and 0; every other token an ordinary one."""
+    rows, x, dt, a, b, c, kw = scan_inputs(251, [130, 64], 3, 1, 32, 48, dtype)
+    dt = dt.clone()
+    dt[::2] = -80 - 30 * torch.arange(dt[::2].numel(), device="cuda").view_as(dt[::2]).float().remainder(31).div(31).to(dt.dtype)
+    kw.pop("dt_bias")
+    got, _ = check_scan(rows, x, dt, a, b, c, kw)
+    assert bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_a_masked_token_that_is_not_finite_spoils_what_the_recurrence_says(dtype):
+    """0 times a NaN is one: a mask is for tokens of finite x and b.  What is not finite in x spoils its channel from there on, beside and before it nothing."""
+    rows, x, dt, a, b, c, kw = scan_inputs(252, [70], 3, 1, 32, 48, dtype)
+    dt, spoilt = dt.clone(), x.clone()
+    dt[40] = -np.inf
+    clean = ssm().selective_scan(x, dt, a, b, c, rows, **kw)
+    spoilt[40, 1, 3] = np.nan
+    got = ssm().selective_scan(spoilt, dt, a, b, c, rows, **kw)
+    hit = torch.zeros(x.shape, dtype=torch.bool, device="cuda")
+    hit[40:, 1, 3] = True
+    assert torch.equal(got[~hit], clean[~hit]) and bool(torch.isnan(got[hit]).all())
