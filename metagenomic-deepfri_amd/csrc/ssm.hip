@@ -235,9 +235,11 @@ __global__ __launch_bounds__(256, W <= 3 ? 3 : W <= 7 ? 2 : 1) void k_conv(mdf_c
 // the reads of B^T that its registers are k in their natural order and C is read as it lies.  (B C^T) comes out transposed,
 // lane = i, and so does Y: a lane holds four consecutive channels of a row, which leave in 16-byte stores (with a swap between the halves for 16-bit types).
 // X comes in 16-byte loads through a tile in LDS; it and B^T are read from their rows by the transposing read.
-// Operands are sums of bfloat16 terms: bfloat16 inputs are one, float16 two and float32, M, S and what goes into the state three (all exact); of two such sums the
-// term products below 2^-24 are left out.  So for every type the arithmetic is that of float32, and a 16-bit output is rounded once.  (M and S in two terms, 2^-16,
-// took 324 us in place of 360 in the case below, and left its bfloat16 outputs 1.2e-4 in the 2-norm off float32 products rounded once; now 2.3e-5.)
+// Operands are sums of bfloat16 terms: bfloat16 inputs are one, float16 two and float32, M, S and what goes into the state three (all exact).  Of the term products
+// of two such sums those below 2^-24 are left out -- none where one of the two is bfloat16; elsewhere the second of three terms is rounded, so that what is left out
+// has no sign of its own (48 float32 sequences, off 64 bits: 1.32e-7 -> 1.19e-7 at the same time; 1.19e-7 too with two more products and 9 % more time).  So for
+// every type the arithmetic is that of float32, and a 16-bit output is rounded once.  (M and S in two terms, 2^-16, took 324 us in place of 360 in the case
+// below, and left its bfloat16 outputs 1.2e-4 in the 2-norm off those of float32 products; now 2.3e-5.)
 // Bound for bfloat16 by issue: per chunk and wave about 780 vector and 52 matrix instructions (state_dim 128), which hardly overlap with two waves per SIMD.  128 sequences
 // of 512 rows, 32 heads of 64 x 128: 300 to 327 us from card to card (its bytes would take 113); 257 without the matrix instructions, 287 without splitting S, M and W into terms.
 // Measured there: 8 waves a workgroup 335, three waves per SIMD 590 (spills), matrix and vector instructions woven by hand 346.
@@ -255,12 +257,19 @@ __device__ __forceinline__ unsigned cvt_pk_bf16(float a, float b)
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, b2));
 }
 // Two values -> TERMS packed bf16 pairs whose sum they are: each term takes the leading 8 bits of what the ones before leave over (cut off, not rounded:
-// one v_perm for the pair), so three terms are exact for float32, two for float16.
-template <int TERMS>
+// one v_perm for the pair), so three terms are exact for float32, two for float16.  ROUND: the second of three is rounded to nearest (a conversion for the pair, and
+// no overflow as there would be with the first): the third, exact still, is half as large and of either sign, and so are the products of terms that are left out.
+template <int TERMS, bool ROUND = false>
 __device__ __forceinline__ void split_pair(float a, float b, unsigned (&o)[TERMS])
 {
 #pragma unroll
     for (int i = 0; i < TERMS; ++i) {
+        if (ROUND && TERMS == 3 && i == 1) {
+            o[i] = cvt_pk_bf16(a, b);
+            a -= __uint_as_float(o[i] << 16);
+            b -= __uint_as_float(o[i] & 0xffff0000u);
+            continue;
+        }
         o[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);   // the upper halves
         if (i + 1 < TERMS) {
             a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
@@ -268,13 +277,13 @@ __device__ __forceinline__ void split_pair(float a, float b, unsigned (&o)[TERMS
         }
     }
 }
-template <int TERMS>
+template <int TERMS, bool ROUND = false>
 __device__ __forceinline__ void split8(const float *v, u32x4 (&o)[TERMS])
 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         unsigned u[TERMS];
-        split_pair<TERMS>(v[2 * i], v[2 * i + 1], u);
+        split_pair<TERMS, ROUND>(v[2 * i], v[2 * i + 1], u);
 #pragma unroll
         for (int k = 0; k < TERMS; ++k) o[k][i] = u[k];
     }
@@ -311,7 +320,7 @@ template <typename T> struct Chunk {   // float
     __device__ __forceinline__ bool finite(int i) const { return fabsf(v[i]) < __builtin_inff(); }
     __device__ __forceinline__ void clear(int i) { v[i] = 0.0f; }
     __device__ __forceinline__ float get(int i) const { return v[i]; }
-    template <int N> __device__ __forceinline__ void terms(int kb, u32x4 (&o)[N]) const { split8<N>(v + 8 * kb, o); }
+    template <int N> __device__ __forceinline__ void terms(int kb, u32x4 (&o)[N]) const { split8<N, true>(v + 8 * kb, o); }
 };
 template <typename T> struct Packed {   // pairs of 16-bit values
     u32x4 v[2];
@@ -600,7 +609,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
                     float f[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] = to_f32(v.v[e]);
-                    split8<TX>(f, u);
+                    split8<TX, true>(f, u);
                 }
 #pragma unroll
                 for (int x = 0; x < TX; ++x) {
@@ -660,7 +669,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
                 float sv[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sv[e] = S[kb / 2][8 * (kb & 1) + e];
-                split8<3>(sv, sf);
+                split8<3, TX != 1>(sv, sf);
                 product<K::IN>(G, bf, cf);     // lane = row i of C, registers = j
                 product<2>(Y, sf, cf);    // lane = row i, registers = channels
             }
@@ -681,7 +690,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 u32x4 mf[3];
-                split8<3>(m + 8 * kb, mf);
+                split8<3, TX != 1>(m + 8 * kb, mf);
                 product<2>(Y, X[kb], mf);
             }
         }
@@ -696,7 +705,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             }
             if (bad < SCAN_Q) w[0] = __builtin_nanf("");
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) split8<3>(w + 8 * kb, W[kb]);
+            for (int kb = 0; kb < 2; ++kb) split8<3, TX != 1>(w + 8 * kb, W[kb]);
             const float decay = st[4][SCAN_Q - 1];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
