@@ -235,3 +235,71 @@ def test_scan_of_float32_products_leans_to_no_side():
     assert error.numel() == 2**17 and float(error.abs().max()) < 2.0**-21
     mean = float(error.mean())
     assert abs(mean) < 2.0**-27, mean
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# large arrays, replayed graphs
+# ---------------------------------------------------------------------------------------------------------------------
+def test_rows_behind_32_bit_offsets():
+    """Sequences at the end of arrays of more than 2^32 bytes and 2^31 values: the same bits as in an array of their own."""
+    S, lens, R = ssm(), [600, 3], 1_050_000
+    g = torch.Generator(device="cuda").manual_seed(271)
+    heads, head_dim, state_dim = 32, 64, 64
+    ch, n = heads * head_dim, sum(lens)
+    small = torch.randn(n, ch, generator=g, device="cuda").bfloat16()
+    bc, dt = torch.randn(n, 2, state_dim, generator=g, device="cuda").bfloat16(), torch.randn(n, heads, generator=g, device="cuda")
+    a, weight, gain = -torch.rand(heads, generator=g, device="cuda") * 4 - 1, torch.randn(4, ch, generator=g, device="cuda"), torch.rand(ch, generator=g, device="cuda")
+    big, out = torch.zeros(R, ch, dtype=torch.bfloat16, device="cuda"), torch.empty(R, ch, dtype=torch.bfloat16, device="cuda")
+    big[R - n:] = small
+    big_bc, big_dt = torch.zeros(R, 2, state_dim, dtype=torch.bfloat16, device="cuda"), torch.zeros(R, heads, device="cuda")
+    big_bc[R - n:], big_dt[R - n:] = bc, dt
+    own = S.SequenceRows.build(lens)
+    far = S.SequenceRows(own.lengths, own.row_off + (R - n), own.max_len)
+    heads_of = lambda t: t.view(-1, heads, head_dim)  # noqa: E731
+    want = S.selective_scan(heads_of(small), dt, a, bc[:, :1], bc[:, 1:], own).flatten(1)
+    S.selective_scan(heads_of(big), big_dt, a, big_bc[:, :1], big_bc[:, 1:], far, out=heads_of(out))
+    slack = 2.0**-7 * want.float().abs() + 2e-5 * float(want.float().abs().max())      # cut into other segments: float32 sums in another order may round to the next bfloat16
+    assert bool(((out[R - n:].float() - want.float()).abs() <= slack).all())
+    want = S.causal_conv(small, weight, own)
+    S.causal_conv(big, weight, far, out=out)
+    assert torch.equal(out[R - n:], want)
+    _, want = S.block_norm(small, post_weight=gain)
+    S.block_norm(big, post_weight=gain, out=out)
+    assert torch.equal(out[R - n:], want)
+
+
+def test_a_captured_scan_replayed_with_other_lengths():
+    """The cut is sized on the host by max_len; which rows are whose is read on the GPU: one graph for every mix of lengths in the same rows, with eager work and other
+    graphs' workspaces between the replays."""
+    S = ssm()
+    R = 2100
+    _, x, dt, a, b, c, kw = scan_inputs(281, [R], 2, 1, 32, 48, "f32")
+    mixes = [[2000, 60, 40], [700, 1400, 0], [3, 900, 1197], [0, 0, 2100], [100, 100, 100]]
+    lengths, off = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    rows = S.SequenceRows(lengths, off, 2100)
+    call = lambda: S.selective_scan(x, dt, a, b, c, rows, **kw)  # noqa: E731
+
+    def fill(lens):
+        own = S.SequenceRows.build(lens)
+        lengths.copy_(own.lengths), off.copy_(own.row_off)
+
+    fill(mixes[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(call())
+    for lens in mixes + mixes[::-1]:
+        fill(lens)
+        for graph in graphs:
+            graph.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager)
+        assert bool((eager[sum(lens):] == 0).all())
+        want, slack, _ = orc.scan(f64(x), f64(dt), f64(a), f64(b), f64(c), lens, off.tolist(), d=f64(kw["d"]), dt_bias=f64(kw["dt_bias"]))
+        near(eager, want, slack)
