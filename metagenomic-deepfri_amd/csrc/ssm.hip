@@ -237,12 +237,14 @@ __global__ __launch_bounds__(256, W <= 3 ? 3 : W <= 7 ? 2 : 1) void k_conv(mdf_c
 // X comes in 16-byte loads through a tile in LDS; it and B^T are read from their rows by the transposing read.
 // Operands are sums of bfloat16 terms: bfloat16 inputs are one, float16 two and float32, M, S and what goes into the state three (all exact).  Of the term products
 // of two such sums those below 2^-24 are left out -- none where one of the two is bfloat16; elsewhere the second of three terms is rounded, so that what is left out
-// has no sign of its own (48 float32 sequences, off 64 bits: 1.32e-7 -> 1.19e-7 at the same time; 1.19e-7 too with two more products and 9 % more time).  So for
+// has no sign of its own (48 float32 sequences, off 64 bits: 1.32e-7 -> 1.19e-7 in the same time; two more products give 1.19e-7 too, in 9 % more).  So for
 // every type the arithmetic is that of float32, and a 16-bit output is rounded once.  (M and S in two terms, 2^-16, took 324 us in place of 360 in the case
 // below, and left its bfloat16 outputs 1.2e-4 in the 2-norm off those of float32 products; now 2.3e-5.)
-// Bound for bfloat16 by issue: per chunk and wave about 780 vector and 52 matrix instructions (state_dim 128), which hardly overlap with two waves per SIMD.  128 sequences
-// of 512 rows, 32 heads of 64 x 128: 300 to 327 us from card to card (its bytes would take 113); 257 without the matrix instructions, 287 without splitting S, M and W into terms.
-// Measured there: 8 waves a workgroup 335, three waves per SIMD 590 (spills), matrix and vector instructions woven by hand 346.
+// Bound for bfloat16 by work that hardly overlaps with two waves per SIMD: per chunk and wave about 980 vector and 62 matrix instructions (state_dim 128) and the
+// rows of X and Y.  128 sequences of 512 rows, 32 heads of 64 x 128: 346 to 360 us from card to card (its bytes would take 113); 263 without the matrix instructions,
+// 303 without splitting S, M and W into terms, 270 without loading X and storing Y.  Some of it is made more than once: G = B C^T by each of the four waves (8 of the
+// 62), M by both waves of a 64-channel head.  float16 takes 650 there, float32 850: one wave per SIMD.
+// Measured with two terms of S and M, at 319 to 337: 8 waves a workgroup 335, three waves per SIMD 590 (spills), matrix and vector instructions woven by hand 346.
 // Long sequences are cut into segments when there are too few (sequence, head) pairs to fill the GPU: a first launch makes each segment's state from zero
 // (STATE: no Y, no C), a small one carries the states from segment to segment, the last one makes Y.
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -423,7 +425,7 @@ struct ScanSplit {
 __device__ __forceinline__ int slot_owner(const mdf_seq_rows &r, const ScanSplit &cut, int slot) { return seq_before(r.row_off, r.B, (int64_t)(slot + 1) * (cut.rows / 2) - 1); }
 
 // WORDS: every row of x, b and c, and every head's and group's part of it, begins on a word.  A template, since the choice inside the loop cost aligned calls 375 us
-// in place of 319 (128 x 512 rows as above); unaligned ones load whole words and shift them.
+// in place of 319 (128 x 512 rows as above, two terms of S and M); unaligned ones load whole words and shift them.
 template <typename T, int NT, bool STATE, bool WORDS>
 __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2) void k_scan(mdf_scan_args g, ScanSplit cut, int items, int unit_blocks)
 {
@@ -629,7 +631,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, Terms<T>::X > 1 && NT > 2 ? 1 : 2)
             }
     };
     // Loads are waited for in the order they and the stores were issued, so a chunk is staged in front of the stores of the one before it: behind them it would
-    // wait for their way to memory too, once per chunk (346 -> 337 us).
+    // wait for their way to memory too, once per chunk (346 -> 337 us, two terms of S and M).
     request(first);
     request_dt(first);
     decays(first);
