@@ -927,6 +927,13 @@ __device__ __forceinline__ float row_sum(float v, float *part)
     return v;
 }
 
+// v / d for many v at two instructions each: the reciprocal and what it is off by, so the quotient is rounded once (a lone reciprocal rounds twice)
+struct Reciprocal {
+    float q, rest;
+    __device__ __forceinline__ explicit Reciprocal(float d) : q(1.0f / d), rest(d < __builtin_inff() ? fmaf(-d, q, 1.0f) * q : 0.0f) {}
+    __device__ __forceinline__ float times(float v) const { return fmaf(v, q, v * rest); }
+};
+
 // thread t of a row holds the 8 values from (v TPR + t) 8 on; a row's last few are taken one by one
 template <typename T, typename R, int TPR, int VPT>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_block_norm(mdf_block_norm_args g)
@@ -980,14 +987,13 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_block_norm(mdf_block_
     };
     // values beyond the row are zeros going in; the centred sum of squares leaves them out again
     auto norm = [&](const float *weight, const float *bias) {
-        const float inv = 1.0f / (float)width;
         float mean = 0.0f, sum = 0.0f;
         if (g.center) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) mean += x[v][e];
-            mean = row_sum<TPR>(mean, part) * inv;
+            mean = row_sum<TPR>(mean, part) / (float)width;
         }
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
@@ -996,13 +1002,13 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_block_norm(mdf_block_
                 if (e < left(v)) x[v][e] -= mean;
                 sum = fmaf(x[v][e], x[v][e], sum);
             }
-        const float q = 1.0f / sqrtf(row_sum<TPR>(sum, part) * inv + g.eps);
+        const Reciprocal q(sqrtf(row_sum<TPR>(sum, part) / (float)width + g.eps));
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             Raw<float, 8> w = param(weight, v), o = {};
             if (bias) o = param(bias, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[v][e] = fmaf(x[v][e] * q, w.v[e], o.v[e]);
+            for (int e = 0; e < 8; ++e) x[v][e] = fmaf(q.times(x[v][e]), w.v[e], o.v[e]);
         }
     };
     auto store = [&](auto *p) {
@@ -1057,7 +1063,8 @@ __global__ __launch_bounds__(256) void k_block_norm_walk(mdf_block_norm_args g)
         return g.gate_act == MDF_ACT_SILU ? silu(z) : g.gate_act == MDF_ACT_SIGMOID ? sigmoid(z) : z;
     };
     auto first = [&](int c) { return to_f32(s[c]) * (gate && g.gate_first ? gated(c) : 1.0f); };
-    float m1 = 0.0f, q1 = 1.0f, m2 = 0.0f, q2 = 1.0f, sum = 0.0f;
+    float m1 = 0.0f, m2 = 0.0f, sum = 0.0f;
+    Reciprocal q1(1.0f), q2(1.0f);
     if (g.post_weight) {
         if (g.center) {
             for (int c = c0 + threadIdx.x; c < c1; c += 256) sum += first(c);
@@ -1065,11 +1072,11 @@ __global__ __launch_bounds__(256) void k_block_norm_walk(mdf_block_norm_args g)
         }
         sum = 0.0f;
         for (int c = c0 + threadIdx.x; c < c1; c += 256) sum += (first(c) - m1) * (first(c) - m1);
-        q1 = 1.0f / sqrtf(block_sum(sum) / width + g.eps);
+        q1 = Reciprocal(sqrtf(block_sum(sum) / width + g.eps));
     }
     auto after = [&](int c) {
         float v = first(c);
-        if (g.post_weight) v = (v - m1) * q1 * g.post_weight[c] + (g.post_bias ? g.post_bias[c] : 0.0f);
+        if (g.post_weight) v = q1.times(v - m1) * g.post_weight[c] + (g.post_bias ? g.post_bias[c] : 0.0f);
         if (gate && !g.gate_first) v *= gated(c);
         return res ? to_f32(res[c]) + g.scale * (g.scale_vec ? g.scale_vec[c] : 1.0f) * v : v;
     };
@@ -1081,12 +1088,12 @@ __global__ __launch_bounds__(256) void k_block_norm_walk(mdf_block_norm_args g)
         }
         sum = 0.0f;
         for (int c = c0 + threadIdx.x; c < c1; c += 256) sum += (after(c) - m2) * (after(c) - m2);
-        q2 = 1.0f / sqrtf(block_sum(sum) / width + g.eps);
+        q2 = Reciprocal(sqrtf(block_sum(sum) / width + g.eps));
     }
     for (int c = c0 + threadIdx.x; c < c1; c += 256) {
         const float v = after(c);
         if (res) static_cast<R *>(g.residual_out)[row * g.ldro + c] = from_f32<R>(v);
-        if (g.pre_weight) static_cast<T *>(g.out)[row * g.ldo + c] = from_f32<T>((v - m2) * q2 * g.pre_weight[c] + (g.pre_bias ? g.pre_bias[c] : 0.0f));
+        if (g.pre_weight) static_cast<T *>(g.out)[row * g.ldo + c] = from_f32<T>(q2.times(v - m2) * g.pre_weight[c] + (g.pre_bias ? g.pre_bias[c] : 0.0f));
         else if (!res) static_cast<T *>(g.out)[row * g.ldo + c] = from_f32<T>(v);
     }
 }
@@ -1118,7 +1125,7 @@ static void norm_launch(const mdf_block_norm_args &a, hipStream_t st)
 }
 // As few threads as hold the row in one vector each, to 512 of them; then two vectors.  128 Mi bfloat16 values in rows of `width` with a gate, us:
 //   512: 64 threads x 1 vector 145-158, 128 x 1 231-246        1 024: 128 x 1 144, 64 x 2 166, 256 x 1 233       2 048: 256 x 1 143, 128 x 2 160, 64 x 4 311, 512 x 1 255
-//   4 096: 512 x 1 152, 256 x 2 188, 1 024 x 1 383             8 192: 512 x 2 200, 1 024 x 1 228, 256 x 4 301    16 384: 1 024 x 2 210, the walk 500
+//   4 096: 512 x 1 152, 256 x 2 188, 1 024 x 1 383             8 192: 512 x 2 200, 1 024 x 1 228, 256 x 4 301    16 384: 1 024 x 2 215, the walk 500
 template <typename T, typename R>
 static void norm_by_width(const mdf_block_norm_args &a, hipStream_t st)
 {

@@ -303,3 +303,24 @@ def test_a_captured_scan_replayed_with_other_lengths():
         assert bool((eager[sum(lens):] == 0).all())
         want, slack, _ = orc.scan(f64(x), f64(dt), f64(a), f64(b), f64(c), lens, off.tolist(), d=f64(kw["d"]), dt_bias=f64(kw["dt_bias"]))
         near(eager, want, slack)
+
+
+@pytest.mark.parametrize("dim", [64, 2048, 32768])
+def test_norm_of_equal_values_is_one(dim):
+    """Rows of k, k, k, ...: squares, sums, mean and root are exact (k <= 256 and a power of two of them: partial sums stay below 2^24 times a power of two), so the
+    quotient is 1 to the last bit, which k times a rounded 1 / k is not for one k in seven."""
+    k = torch.arange(1, 257, device="cuda").float()
+    s = (k * torch.tensor([1.0, -1.0], device="cuda").repeat(128)).unsqueeze(1).expand(256, dim).contiguous()
+    w = torch.rand(dim, device="cuda") + 0.5
+    _, got = ssm().block_norm(s, post_weight=w, eps=0.0)
+    assert torch.equal(got, torch.sign(s) * w)
+    r, got = ssm().block_norm(s, residual=torch.zeros_like(s), pre_weight=w, eps=0.0)
+    assert torch.equal(r, s) and torch.equal(got, torch.sign(s) * w)
+
+
+def test_norm_of_rows_whose_squares_leave_the_range_is_no_nan():
+    """Mean square infinite: 0, as 1 / infinity says; an infinity among the values is a NaN in its own place."""
+    s = torch.full((2, 128), 1e30, device="cuda")
+    s[1, 5] = np.inf
+    _, got = ssm().block_norm(s, post_weight=torch.ones(128, device="cuda"))
+    assert bool((got[0] == 0).all()) and bool(torch.isnan(got[1, 5])) and bool((got[1, :5] == 0).all()) and bool((got[1, 6:] == 0).all())
