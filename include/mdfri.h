@@ -277,7 +277,8 @@ int mdf_causal_conv_dev(const mdf_conv_args *args, void *stream);
  * contiguous inside a row, row strides at least a row's width; dt (R, heads) of any of the three types.  y must not overlap an input.  head_dim 1..256, state_dim 1..128.
  * dt of -infinity (D = 0) passes the state on unchanged if the token's x and b are finite.  Non-finite values stay where the recurrence puts them: nothing before
  * the token or beside the channel they enter by is touched (an infinity may come out as NaN).  Two tokens' b . c is formed in front of decays and step sizes: where
- * it leaves float32's range, y does, however small these would make it.  Sequences (and 1 024 segments of long ones) times groups times a quarter of a group's blocks of 32 channels: below 2^31. */
+ * it leaves float32's range, y does, however small these would make it.  Rows and their strides: below 2^23 values.  Sequences (and 1 024 segments of long
+ * ones) times groups times a quarter of a group's blocks of 32 channels: below 2^31. */
 typedef struct {
     mdf_seq_rows rows;
     const void *x, *b, *c, *dt;

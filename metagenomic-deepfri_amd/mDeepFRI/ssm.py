@@ -156,9 +156,11 @@ def _indices(t, name: str, device, count: int):
     return t.data_ptr()
 
 
-def _state(t, name: str, device, dtype, tail: tuple):
+def _state(t, name: str, device, dtype, tail: tuple, count: int):
     if t.dtype != dtype or tuple(t.shape[1:]) != tail or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {('*',) + tail} on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    if count and not t.shape[0]:                   # (its address is none: the library would take it for a call without states)
+        raise ValueError(f"{name} has no slot for any of {count} sequences")
     if t.requires_grad and _torch().is_grad_enabled():
         raise ValueError(f"{name} asks for a gradient: the state-space operators are inference only")
 
@@ -272,7 +274,7 @@ def causal_conv(x, weight, rows: SequenceRows, *, bias=None, silu: bool = True, 
         _vector(weight, "weight", device, (width, channels)), _vector(bias, "bias", device, (channels,))
         _check_rows(a.rows, rows, device, x.shape[0], slots, positions, state)
         if state is not None:
-            _state(state, "state", device, x.dtype, (width, channels))
+            _state(state, "state", device, x.dtype, (width, channels), rows.count)
         _check_out(out, x)
         a.ldo = channels if out is None else _matrix(out, "out", device, (channels,), x.shape[0])
         a.channels, a.width, a.dtype, a.silu, a.zero_skipped = channels, width, code, bool(silu), out is None
@@ -313,7 +315,7 @@ def selective_scan(x, dt, a, b, c, rows: SequenceRows, *, d=None, dt_bias=None, 
             _vector(v, name, device, (heads,))
         _check_rows(g.rows, rows, device, total, slots, positions, state)
         if state is not None:
-            _state(state, "state", device, _torch().float32, (heads, head_dim, state_dim))
+            _state(state, "state", device, _torch().float32, (heads, head_dim, state_dim), rows.count)
         _check_out(out, x)
         g.ldy = heads * head_dim if out is None else _matrix(out, "out", device, (heads, head_dim), total)
         g.heads, g.groups, g.head_dim, g.state_dim, g.zero_skipped = heads, groups, head_dim, state_dim, out is None
@@ -353,8 +355,8 @@ def selective_step(xbc, dt, a, *, conv_weight, conv_state, state, positions=None
         _vector(conv_weight, "conv_weight", device, (width, channels)), _vector(conv_bias, "conv_bias", device, (channels,))
         for name, v in (("a", a), ("d", d), ("dt_bias", dt_bias)):
             _vector(v, name, device, (heads,))
-        _state(conv_state, "conv_state", device, xbc.dtype, (width, channels))
-        _state(state, "state", device, _torch().float32, (heads, head_dim, state_dim))
+        _state(conv_state, "conv_state", device, xbc.dtype, (width, channels), n)
+        _state(state, "state", device, _torch().float32, (heads, head_dim, state_dim), n)
         if conv_state.shape[0] != state.shape[0]:
             raise ValueError(f"{conv_state.shape[0]} convolution states beside {state.shape[0]} scan states")
         _indices(slots, "slots", device, n), _indices(positions, "positions", device, n)

@@ -188,3 +188,21 @@ def test_checked_tensors_of_rows_cannot_be_exchanged():
     assert rows.lengths.tolist() == [3, 0, 5] and rows.row_off.tolist() == [0, 3, 3, 8] and rows.count == 3 and rows.form == (3, -1)
     rows.max_len = 7                                  # another batch of three in the same tensors
     assert rows.max_len == 7
+
+
+@pytest.mark.parametrize("op", ["causal_conv", "selective_scan", "selective_step"])
+def test_a_pool_without_slots_is_refused(op, monkeypatch):
+    """An empty tensor has no address, which to the library is a call without states: it would run what has to be skipped."""
+    import torch
+    monkeypatch.setattr(ssm, "_matrix", lambda t, *a: t.stride(0))
+    monkeypatch.setattr(ssm, "_call", lambda fn, device, *args: None)
+    fn, args, more = _calls()[op]
+    args = {**args, **more}
+    fn(**args)
+    for name in ("state", "conv_state"):
+        if name in args:
+            with pytest.raises(ValueError, match="no slot"):
+                fn(**{**args, name: args[name][:0], "slots": torch.full((2,), -1, dtype=torch.int32)})
+    if op != "selective_step":
+        nobody = dict(args, rows=ssm.SequenceRows.build([], device="cpu"), state=args["state"][:0])
+        assert torch.equal(fn(**nobody), args["out"])
